@@ -10,7 +10,7 @@ The operators, for a tensor x of which one dimension of length L is normalised:
 * dropout: element (or unit) j is kept when u_j >= round(p * 2^32), u_j being word j % 4 of the Philox4x32-10
   block with key ``seed`` and counter (j // 4, sequence), both 64 bits wide, low word first;
   y = x / (1 - p) where kept, 0 elsewhere, plus the residual where there is one;
-* the join: h = residual + dropout(x), rounded to the type of x, and y = layer norm of that h.
+* the join: h = residual + dropout(x), a 32-bit sum rounded to the type of x, and y = layer norm of that h.
 """
 
 from __future__ import annotations
@@ -301,9 +301,10 @@ def exact(case, seed):
         if "residual" in wide:
             x = x + wide["residual"]
     if case["op"] == "join":
-        # the norm is of h as it is returned: rounded, with the gradient passed on as it is
-        h = x + (x.detach().to(state["x"].dtype).double() - x.detach())
-        outputs = [norm(h), h]
+        # the norm is of h as it is returned, a 32-bit sum rounded to its type, with the gradient passed on as it is
+        scaled = state["x"].detach().float() * (1 / (1 - case["p"]))
+        rounded = (state["residual"].detach().float() + torch.where(kept.view(x.shape), scaled, 0.0)).to(state["x"].dtype)
+        outputs = [norm(x + (rounded.double() - x.detach())), x]
     else:
         outputs = [norm(x) if case["op"] == "layer_norm" else x]
     if not case["train"]:
