@@ -18,6 +18,7 @@
 #include "separable.cuh"
 #include "gather_pull.cuh"
 #include "gather_stream.cuh"
+#include "host_guard.h"
 
 namespace serron {
 // compile-time-K separable kernels, instantiated per storage type in sep_fast_<type>.cu; they return
@@ -54,60 +55,6 @@ namespace {
 
 thread_local std::string g_last_error;
 
-struct Failure {
-    int code;
-    std::string message;
-};
-
-template <typename... Args>
-std::string concat(const Args&... args) {
-    std::ostringstream oss;
-    ((oss << args), ...);
-    return oss.str();
-}
-
-#define SB_CHECK(cond, ...)                                                  \
-    do {                                                                     \
-        if (!(cond)) throw Failure{SERRON_ERR_INVALID, concat(__VA_ARGS__)}; \
-    } while (0)
-
-#define SB_CUDA(expr)                                                                                         \
-    do {                                                                                                      \
-        const cudaError_t err_ = (expr);                                                                      \
-        if (err_ != cudaSuccess)                                                                              \
-            throw Failure{SERRON_ERR_CUDA, concat("serron: CUDA error ", cudaGetErrorName(err_), ": ",      \
-                                                  cudaGetErrorString(err_), " (", #expr, ")")};              \
-    } while (0)
-
-template <typename F>
-int guarded(F&& f) {
-    try {
-        f();
-        return SERRON_OK;
-    } catch (const Failure& e) {
-        g_last_error = e.message;
-        return e.code;
-    } catch (const std::exception& e) {
-        g_last_error = e.what();
-        return SERRON_ERR_INVALID;
-    }
-}
-
-// Makes `device` current for the scope of a call and restores the previous device.
-struct DeviceScope {
-    int previous = -1;
-    explicit DeviceScope(int device) {
-        if (cudaGetDevice(&previous) != cudaSuccess) previous = -1;
-        cudaGetLastError();
-        if (previous != device) SB_CUDA(cudaSetDevice(device));
-    }
-    ~DeviceScope() {
-        int now = -1;
-        if (previous >= 0 && cudaGetDevice(&now) == cudaSuccess && now != previous) cudaSetDevice(previous);
-    }
-};
-
-size_t elem_size(int dtype) { return dtype == kF64 ? 8 : dtype == kF32 ? 4 : 2; }
 size_t acc_size(int dtype) { return dtype == kF64 ? 8 : 4; }
 
 struct DeviceInfo {
