@@ -211,6 +211,65 @@ SERRON_API int serron_derived_forward(int32_t mode, const void* input, const int
                                       int32_t winners_format, int32_t device, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Layer operators: what a network puts around the learnable morphology layers.  No reference counterpart.
+ *
+ * Layer norm over one dimension of a dense tensor seen as (outer, len, inner): each of the outer * inner
+ * rows (the len elements x[o, :, i], `inner` apart) becomes (x - mean) / sqrt(var + eps) * weight + bias,
+ * var the mean of (x - mean)^2.  An image (N, C, H, W) normalised over its channels at every pixel is
+ * (N, C, H * W); tokens (rows, len) are (rows, len, 1).
+ *   - `weight` and `bias` (len elements each; either may be NULL) are float32 or of the input's dtype, as
+ *     `param_dtype` says for both.
+ *   - `mean` and `rstd` (outer * inner elements, row (o, i) at o * inner + i; float32, or float64 for
+ *     float64 inputs) are what the backward reads; both may be NULL where none follows.
+ *   - the backward gives grad_input, grad_weight and grad_bias (the last two of `param_dtype`), each
+ *     skipped where NULL, in sums whose order depends on the sizes alone.
+ *   - workspace: serron_layer_norm_workspace_bytes bytes, 256-byte aligned; -1 (with a message) for
+ *     arguments no call takes.
+ *
+ * Dropout: y = residual + (kept ? input / (1 - p) : 0), `residual` NULL for none.  Each run of `span`
+ * consecutive elements shares one decision (1: every element; H * W: whole channels; C * H * W: whole
+ * samples).  Decision j keeps its run when word j % 4 of the Philox4x32-10 block with counter
+ * (j / 4, sequence) and key `seed` (64 bits each, low word first) is at least round(p * 2^32).  The mask
+ * depends on nothing else and is not stored: the backward is the same call over grad_output, without
+ * the residual.  `seed_device`, where set, is the device address of a 64-bit seed that the kernel
+ * reads in place of `seed` (so that a captured graph can be replayed under another seed).  A dropped element is 0 (plus
+ * the residual) whatever it held, and p = 1 drops every one.
+ *
+ * The join of both at the end of a residual branch: sum = residual + dropout(input) (decisions by
+ * element, in the order of memory; rounded to `dtype`), output = layer norm of that sum.  Its backward
+ * takes the gradients of both outputs (`grad_sum` NULL for none) and gives those of both inputs
+ * (each skipped where NULL).  Workspace: serron_layer_norm_workspace_bytes.
+ * --------------------------------------------------------------------------------------------- */
+SERRON_API int64_t serron_layer_norm_workspace_bytes(int64_t outer, int64_t len, int64_t inner, int32_t dtype,
+                                                     int32_t backward);
+SERRON_API int serron_layer_norm(const void* input, int64_t outer, int64_t len, int64_t inner, int32_t dtype,
+                                 const void* weight, const void* bias, int32_t param_dtype, double eps, void* output,
+                                 void* mean, void* rstd, void* workspace, int64_t workspace_bytes, int32_t device,
+                                 void* stream);
+SERRON_API int serron_layer_norm_backward(const void* grad_output, const void* input, const void* mean,
+                                          const void* rstd, int64_t outer, int64_t len, int64_t inner, int32_t dtype,
+                                          const void* weight, int32_t param_dtype, void* grad_input, void* grad_weight,
+                                          void* grad_bias, void* workspace, int64_t workspace_bytes, int32_t device,
+                                          void* stream);
+SERRON_API int serron_dropout(const void* input, const void* residual, int64_t numel, int64_t span, int32_t dtype,
+                              double p, uint64_t seed, const void* seed_device, uint64_t sequence, void* output,
+                              int32_t device, void* stream);
+SERRON_API int serron_dropout_add_layer_norm(const void* input, const void* residual, int64_t outer, int64_t len,
+                                             int64_t inner, int32_t dtype, const void* weight, const void* bias,
+                                             int32_t param_dtype, double p, uint64_t seed, const void* seed_device,
+                                             uint64_t sequence, double eps, void* sum, void* output, void* mean,
+                                             void* rstd, void* workspace, int64_t workspace_bytes, int32_t device,
+                                             void* stream);
+SERRON_API int serron_dropout_add_layer_norm_backward(const void* grad_output, const void* grad_sum, const void* sum,
+                                                      const void* mean, const void* rstd, int64_t outer, int64_t len,
+                                                      int64_t inner, int32_t dtype, const void* weight,
+                                                      int32_t param_dtype, double p, uint64_t seed,
+                                                      const void* seed_device, uint64_t sequence, void* grad_input,
+                                                      void* grad_residual, void* grad_weight, void* grad_bias,
+                                                      void* workspace, int64_t workspace_bytes, int32_t device,
+                                                      void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Algorithm selection.  Replace serron::feasible_algos / heuristic_algo / set_separable_min_k /
  * get_separable_min_k (packages/serron/csrc/bindings.cpp:16-19, gpu/morphology/dispatch_info.cpp:54-81).
  * Return values are as the reference's (bit mask, algorithm code, threshold) or -1 on error.

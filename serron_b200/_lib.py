@@ -57,6 +57,12 @@ EXPORTED = (
     "serron_backward_from_winners_widened",
     "serron_derived_supported",
     "serron_derived_forward",
+    "serron_layer_norm_workspace_bytes",
+    "serron_layer_norm",
+    "serron_layer_norm_backward",
+    "serron_dropout",
+    "serron_dropout_add_layer_norm",
+    "serron_dropout_add_layer_norm_backward",
 )
 
 
@@ -89,6 +95,7 @@ def load() -> ctypes.CDLL:
             )
         lib = ctypes.CDLL(LIB_PATH)
         vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+        u64, f64 = ctypes.c_uint64, ctypes.c_double
         p64 = ctypes.POINTER(ctypes.c_int64)
         lib.serron_last_error.argtypes = []
         lib.serron_last_error.restype = ctypes.c_char_p
@@ -139,6 +146,20 @@ def load() -> ctypes.CDLL:
         lib.serron_forward_autocast.restype = ctypes.c_int
         lib.serron_winners_bytes.argtypes = [p64, i64, i32]
         lib.serron_winners_bytes.restype = i64
+        lib.serron_layer_norm_workspace_bytes.argtypes = [i64, i64, i64, i32, i32]
+        lib.serron_layer_norm_workspace_bytes.restype = i64
+        tail = [vp, i64, i32, vp]  # workspace, its bytes, device, stream
+        drop = [f64, u64, vp, u64]  # p, seed, seed_device, sequence
+        lib.serron_layer_norm.argtypes = [vp, i64, i64, i64, i32, vp, vp, i32, f64, vp, vp, vp, *tail]
+        lib.serron_layer_norm_backward.argtypes = [vp, vp, vp, vp, i64, i64, i64, i32, vp, i32, vp, vp, vp, *tail]
+        lib.serron_dropout.argtypes = [vp, vp, i64, i64, i32, *drop, vp, i32, vp]
+        lib.serron_dropout_add_layer_norm.argtypes = [vp, vp, i64, i64, i64, i32, vp, vp, i32, *drop, f64, vp, vp, vp,
+                                                      vp, *tail]
+        lib.serron_dropout_add_layer_norm_backward.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i32, vp, i32, *drop,
+                                                               vp, vp, vp, vp, *tail]
+        for name in ("serron_layer_norm", "serron_layer_norm_backward", "serron_dropout",
+                     "serron_dropout_add_layer_norm", "serron_dropout_add_layer_norm_backward"):
+            getattr(lib, name).restype = ctypes.c_int
         _lib = lib
         return lib
 

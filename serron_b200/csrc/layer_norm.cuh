@@ -1,0 +1,281 @@
+// Layer norm over one dimension of a dense tensor seen as (outer, len, inner): row r = (o, i) holds the len elements
+// x[o, :, i], `inner` apart.
+//
+//   mean = sum x / len,  rstd = 1 / sqrt(sum (x - mean)^2 / len + eps),  xhat = (x - mean) * rstd
+//   forward    y = xhat * w + b
+//   backward   g = gy * w,  dx = rstd * (g - mean(g) - xhat * mean(g * xhat)),
+//              dw = sum over rows of gy * xhat,  db = sum over rows of gy
+//
+// Statistics and sums are float32 (double for double) whatever the storage type.
+#pragma once
+
+#include "layer_common.cuh"
+
+namespace serron {
+
+struct NormShape {
+    long long rows = 0;  // outer * inner
+    int len = 0, inner = 1;
+
+    // first element of row r; its elements are `inner` apart
+    __device__ __forceinline__ long long base(long long r) const {
+        return inner == 1 ? r * len : (r / inner) * static_cast<long long>(len) * inner + r % inner;
+    }
+};
+
+// ------------------------------------------------------------------------------------------------
+// kernels for any length and layout: rows are cut into chunks of `chunk` elements, each block reduces one chunk of
+// one row (inner == 1: 256 threads along the row) or of 32 neighbouring rows (inner > 1: 32 x 8 threads, neighbouring
+// rows being neighbours in memory), and the chunks' results are joined where they are used.
+// ------------------------------------------------------------------------------------------------
+constexpr int kNormThreads = 256;
+
+// Block-wide sum over the threads of one row: all 256 of a block (ROWS), or the 8 of a column of 32 x 8.
+template <bool ROWS, typename A>
+__device__ __forceinline__ A row_sum(A v, A* shared) {
+    const int t = threadIdx.x;
+    __syncthreads();  // the last use of `shared`
+    if (ROWS) {
+        v = warp_sum(v);
+        if ((t & 31) == 0) shared[t >> 5] = v;
+        __syncthreads();
+        A s = A(0);
+        for (int w = 0; w < kNormThreads / 32; ++w) s += shared[w];
+        return s;
+    }
+    shared[t] = v;
+    __syncthreads();
+    A s = A(0);
+    for (int w = 0; w < kNormThreads / 32; ++w) s += shared[w * 32 + (t & 31)];
+    return s;
+}
+
+// What a thread of the chunk kernels works on.
+struct ChunkPlace {
+    long long row, offset;
+    int first, step, end;
+    bool live;
+};
+template <bool ROWS>
+__device__ __forceinline__ ChunkPlace chunk_place(const NormShape& s, int chunk, int split) {
+    ChunkPlace p;
+    p.row = ROWS ? static_cast<long long>(blockIdx.x) : blockIdx.x * 32ll + (threadIdx.x & 31);
+    p.live = p.row < s.rows;
+    p.offset = p.live ? s.base(p.row) : 0;
+    const long long begin = static_cast<long long>(split) * chunk;
+    p.end = p.live ? static_cast<int>(min(begin + chunk, static_cast<long long>(s.len))) : 0;
+    p.first = static_cast<int>(begin) + (ROWS ? threadIdx.x : threadIdx.x >> 5);
+    p.step = ROWS ? kNormThreads : kNormThreads / 32;
+    return p;
+}
+
+// Mean and sum of squared deviations of each chunk (two passes over it, the second from the caches).
+template <typename T, bool ROWS>
+__global__ void __launch_bounds__(kNormThreads)
+    norm_stats_kernel(const T* __restrict__ x, typename Storage<T>::acc* __restrict__ part, NormShape s, int chunk) {
+    using S = Storage<T>;
+    using A = typename S::acc;
+    __shared__ A shared[kNormThreads];
+    const int split = blockIdx.y;
+    const ChunkPlace p = chunk_place<ROWS>(s, chunk, split);
+    const int count = min(chunk, s.len - split * chunk);
+    A sum = A(0);
+    for (int l = p.first; l < p.end; l += p.step) sum += S::load(x[p.offset + static_cast<long long>(l) * s.inner]);
+    const A mean = row_sum<ROWS>(sum, shared) / A(count);
+    A m2 = A(0);
+    for (int l = p.first; l < p.end; l += p.step) {
+        const A d = S::load(x[p.offset + static_cast<long long>(l) * s.inner]) - mean;
+        m2 += d * d;
+    }
+    m2 = row_sum<ROWS>(m2, shared);
+    if (p.live && (ROWS ? threadIdx.x == 0 : threadIdx.x < 32)) {
+        part[(p.row * gridDim.y + split) * 2] = mean;
+        part[(p.row * gridDim.y + split) * 2 + 1] = m2;
+    }
+}
+
+// Joins the chunks of each row: with count n, mean m and sum of squares q of two parts,
+// m = m1 + (m2 - m1) n2 / n and q = q1 + q2 + (m2 - m1)^2 n1 n2 / n.
+template <typename A>
+__global__ void norm_join_kernel(const A* __restrict__ part, A* __restrict__ mean_out, A* __restrict__ rstd_out,
+                                 NormShape s, int chunk, int splits, double eps) {
+    const long long row = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
+    if (row >= s.rows) return;
+    A mean = part[row * splits * 2], m2 = part[row * splits * 2 + 1], n = A(min(chunk, s.len));
+    for (int k = 1; k < splits; ++k) {
+        const A count = A(min(chunk, s.len - k * chunk));
+        const A d = part[(row * splits + k) * 2] - mean;
+        const A total = n + count;
+        mean += d * (count / total);
+        m2 += part[(row * splits + k) * 2 + 1] + d * d * (n * (count / total));
+        n = total;
+    }
+    mean_out[row] = mean;
+    rstd_out[row] = inverse_root<A>(m2 / A(s.len) + A(eps));
+}
+
+template <typename T, bool ROWS>
+__global__ void __launch_bounds__(kNormThreads)
+    norm_apply_kernel(const T* __restrict__ x, const typename Storage<T>::acc* __restrict__ mean,
+                      const typename Storage<T>::acc* __restrict__ rstd, const void* __restrict__ weight,
+                      const void* __restrict__ bias, bool f32, T* __restrict__ y, NormShape s, int chunk) {
+    using S = Storage<T>;
+    using A = typename S::acc;
+    const ChunkPlace p = chunk_place<ROWS>(s, chunk, blockIdx.y);
+    if (!p.live) return;
+    const A m = mean[p.row], r = rstd[p.row];
+    for (int l = p.first; l < p.end; l += p.step) {
+        const long long e = p.offset + static_cast<long long>(l) * s.inner;
+        A v = (S::load(x[e]) - m) * r;
+        if (weight) v *= load_param<T>(weight, l, f32);
+        if (bias) v += load_param<T>(bias, l, f32);
+        y[e] = S::store(v);
+    }
+}
+
+// Sums of g and g * xhat of each chunk.
+template <typename T, bool ROWS>
+__global__ void __launch_bounds__(kNormThreads)
+    norm_bwd_sums_kernel(const T* __restrict__ gy, const T* __restrict__ x,
+                         const typename Storage<T>::acc* __restrict__ mean,
+                         const typename Storage<T>::acc* __restrict__ rstd, const void* __restrict__ weight, bool f32,
+                         typename Storage<T>::acc* __restrict__ part, NormShape s, int chunk) {
+    using S = Storage<T>;
+    using A = typename S::acc;
+    __shared__ A shared[kNormThreads];
+    const ChunkPlace p = chunk_place<ROWS>(s, chunk, blockIdx.y);
+    const A m = p.live ? mean[p.row] : A(0), r = p.live ? rstd[p.row] : A(0);
+    A s1 = A(0), s2 = A(0);
+    for (int l = p.first; l < p.end; l += p.step) {
+        const long long e = p.offset + static_cast<long long>(l) * s.inner;
+        A g = S::load(gy[e]);
+        if (weight) g *= load_param<T>(weight, l, f32);
+        s1 += g;
+        s2 += g * ((S::load(x[e]) - m) * r);
+    }
+    s1 = row_sum<ROWS>(s1, shared);
+    s2 = row_sum<ROWS>(s2, shared);
+    if (p.live && (ROWS ? threadIdx.x == 0 : threadIdx.x < 32)) {
+        part[(p.row * gridDim.y + blockIdx.y) * 2] = s1;
+        part[(p.row * gridDim.y + blockIdx.y) * 2 + 1] = s2;
+    }
+}
+
+// dx (plus `add`, the gradient that reaches x by another way), and for the join its masked copy `dropped`.
+template <typename T, bool ROWS>
+__global__ void __launch_bounds__(kNormThreads)
+    norm_bwd_apply_kernel(const T* __restrict__ gy, const T* __restrict__ x,
+                          const typename Storage<T>::acc* __restrict__ mean,
+                          const typename Storage<T>::acc* __restrict__ rstd, const void* __restrict__ weight, bool f32,
+                          const typename Storage<T>::acc* __restrict__ part, const T* __restrict__ add,
+                          T* __restrict__ dx, T* __restrict__ dropped, DropRule rule, NormShape s, int chunk) {
+    using S = Storage<T>;
+    using A = typename S::acc;
+    const ChunkPlace p = chunk_place<ROWS>(s, chunk, blockIdx.y);
+    if (!p.live) return;
+    A s1 = A(0), s2 = A(0);
+    for (int k = 0; k < static_cast<int>(gridDim.y); ++k) {
+        s1 += part[(p.row * gridDim.y + k) * 2];
+        s2 += part[(p.row * gridDim.y + k) * 2 + 1];
+    }
+    s1 /= A(s.len);
+    s2 /= A(s.len);
+    const A m = mean[p.row], r = rstd[p.row];
+    for (int l = p.first; l < p.end; l += p.step) {
+        const long long e = p.offset + static_cast<long long>(l) * s.inner;
+        A g = S::load(gy[e]);
+        if (weight) g *= load_param<T>(weight, l, f32);
+        A v = r * (g - s1 - ((S::load(x[e]) - m) * r) * s2);
+        if (add) v += S::load(add[e]);
+        if (dx) dx[e] = S::store(v);
+        if (dropped) {
+            const bool kept = rule.keeps(word_of(philox(e >> 2, rule.sequence, rule.key()), e & 3));
+            dropped[e] = S::store(kept ? scaled<A>(v, A(rule.scale)) : A(0));
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// gradients of weight and bias: sums over rows, first of `rows_per` rows each in A, then of those in double, each in
+// an order that the sizes alone set
+// ------------------------------------------------------------------------------------------------
+
+// inner == 1: a thread owns an element of the row and walks down rows_per rows.
+template <typename T>
+__global__ void __launch_bounds__(kNormThreads)
+    norm_param_rows_kernel(const T* __restrict__ gy, const T* __restrict__ x,
+                           const typename Storage<T>::acc* __restrict__ mean,
+                           const typename Storage<T>::acc* __restrict__ rstd,
+                           typename Storage<T>::acc* __restrict__ part, NormShape s, int rows_per, int tiles) {
+    using S = Storage<T>;
+    using A = typename S::acc;
+    const long long block = blockIdx.x / tiles;
+    const int l = static_cast<int>(blockIdx.x % tiles) * kNormThreads + threadIdx.x;
+    if (l >= s.len) return;
+    const long long first = block * rows_per, end = min(first + rows_per, s.rows);
+    A dw = A(0), db = A(0);
+    for (long long r = first; r < end; ++r) {
+        const A g = S::load(gy[r * s.len + l]);
+        dw += g * ((S::load(x[r * s.len + l]) - mean[r]) * rstd[r]);
+        db += g;
+    }
+    part[(block * 2) * s.len + l] = dw;
+    part[(block * 2 + 1) * s.len + l] = db;
+}
+
+// inner > 1: a block sums rows_per neighbouring rows at one element of them.
+template <typename T>
+__global__ void __launch_bounds__(kNormThreads)
+    norm_param_columns_kernel(const T* __restrict__ gy, const T* __restrict__ x,
+                              const typename Storage<T>::acc* __restrict__ mean,
+                              const typename Storage<T>::acc* __restrict__ rstd,
+                              typename Storage<T>::acc* __restrict__ part, NormShape s, int rows_per) {
+    using S = Storage<T>;
+    using A = typename S::acc;
+    __shared__ A shared[kNormThreads];
+    const long long block = blockIdx.x / s.len;
+    const int l = static_cast<int>(blockIdx.x % s.len);
+    const long long end = min((block + 1) * rows_per, s.rows);
+    A dw = A(0), db = A(0);
+    for (long long r = block * rows_per + threadIdx.x; r < end; r += kNormThreads) {
+        const long long e = s.base(r) + static_cast<long long>(l) * s.inner;
+        const A g = S::load(gy[e]);
+        dw += g * ((S::load(x[e]) - mean[r]) * rstd[r]);
+        db += g;
+    }
+    dw = row_sum<true>(dw, shared);
+    db = row_sum<true>(db, shared);
+    if (threadIdx.x == 0) {
+        part[(block * 2) * s.len + l] = dw;
+        part[(block * 2 + 1) * s.len + l] = db;
+    }
+}
+
+// 32 elements x 8 shares of the partial sums a block.
+template <typename T>
+__global__ void __launch_bounds__(kNormThreads)
+    norm_param_final_kernel(const typename Storage<T>::acc* __restrict__ part, long long blocks, int len,
+                            void* __restrict__ dw, void* __restrict__ db, bool f32) {
+    __shared__ double shared[2][8][32];
+    const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
+    const int l = blockIdx.x * 32 + lane;
+    double w = 0.0, b = 0.0;
+    if (l < len) {
+        for (long long k = share; k < blocks; k += 8) {
+            w += part[k * 2 * len + l];
+            b += part[(k * 2 + 1) * len + l];
+        }
+    }
+    shared[0][share][lane] = w;
+    shared[1][share][lane] = b;
+    __syncthreads();
+    if (share != 0 || l >= len) return;
+    for (int k = 1; k < 8; ++k) {
+        w += shared[0][k][lane];
+        b += shared[1][k][lane];
+    }
+    if (dw) store_param<T>(dw, l, f32, w);
+    if (db) store_param<T>(db, l, f32, b);
+}
+
+}  // namespace serron

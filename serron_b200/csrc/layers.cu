@@ -1,0 +1,309 @@
+// C ABI of the layer operators: layer norm, dropout and their join with a residual sum (layer_norm.cuh, dropout.cuh).
+// Contracts: include/serron_b200.h.
+#include "serron_b200.h"
+
+#include <algorithm>
+#include <cmath>
+#include <limits>
+
+#include "dropout.cuh"
+#include "host_guard.h"
+#include "layer_norm.cuh"
+
+namespace serron {
+namespace {
+
+int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Calls f(T{}) with the storage type of `dtype`.
+template <typename F>
+void with_type(int dtype, F&& f) {
+    switch (dtype) {
+    case kF32: f(float{}); break;
+    case kF64: f(double{}); break;
+    case kF16: f(__half{}); break;
+    default: f(__nv_bfloat16{}); break;
+    }
+}
+
+unsigned grid_of(const char* name, int64_t blocks) {
+    SB_CHECK(blocks < (int64_t(1) << 31), name, ": too large (", blocks, " blocks of work)");
+    return static_cast<unsigned>(blocks);
+}
+
+// ------------------------------------------------------------------------------------------------
+// dropout
+// ------------------------------------------------------------------------------------------------
+DropRule drop_rule(const char* name, double p, uint64_t seed, const void* seed_device, uint64_t sequence) {
+    SB_CHECK(p >= 0.0 && p <= 1.0, name, ": p must be between 0 and 1, got ", p);
+    DropRule rule;
+    rule.seed = seed;
+    rule.seed_device = static_cast<const uint64_t*>(seed_device);
+    rule.sequence = sequence;
+    const double threshold = std::nearbyint(p * 4294967296.0);
+    rule.all = threshold >= 4294967296.0;
+    rule.threshold = rule.all ? 0xffffffffu : static_cast<uint32_t>(threshold);
+    rule.scale = rule.all ? 0.0 : 1.0 / (1.0 - p);
+    return rule;
+}
+
+template <typename T>
+void launch_dropout(const char* name, const void* x, const void* residual, void* y, int64_t n, int64_t span,
+                    const DropRule& rule, cudaStream_t stream) {
+    dropout_kernel<T><<<grid_of(name, ceil_div64(n, 256)), 256, 0, stream>>>(
+        static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<T*>(y), n, span, rule);
+    SB_CUDA(cudaGetLastError());
+}
+
+// ------------------------------------------------------------------------------------------------
+// layer norm
+// ------------------------------------------------------------------------------------------------
+struct Norm {
+    NormShape shape;
+    int chunk = 0, splits = 0;  // a row's cut into chunks
+    int rows_per = 0;           // rows a partial sum of the parameters' gradients covers
+    int64_t blocks = 0;         // such sums
+    int64_t numel() const { return shape.rows * shape.len; }
+};
+
+// Rows per first-level sum of the parameters' gradients: at most 128 additions in a row (32 per thread where a
+// block's threads share a sum), so that the float32 sums stay as exact as a tree's.
+constexpr int kRowsPerSum = 128, kColumnsPerSum = 32 * kNormThreads;
+
+Norm norm_of(const char* name, int64_t outer, int64_t len, int64_t inner) {
+    SB_CHECK(outer >= 0 && inner >= 0, name, ": sizes must be non-negative");
+    SB_CHECK(len >= 1, name, ": the normalised dimension must not be empty");
+    SB_CHECK(len < (int64_t(1) << 31) && inner < (int64_t(1) << 31), name,
+             ": the normalised dimension and the elements behind it must be below 2^31");
+    SB_CHECK(outer == 0 || inner == 0 || outer <= std::numeric_limits<int64_t>::max() / 16 / len / inner, name,
+             ": too many elements");
+    Norm n;
+    n.shape.rows = outer * inner;
+    n.shape.len = static_cast<int>(len);
+    n.shape.inner = static_cast<int>(std::max<int64_t>(inner, 1));
+    n.chunk = static_cast<int>(std::max<int64_t>(inner == 1 ? 8192 : 1024, ceil_div64(len, 65535)));
+    n.splits = static_cast<int>(ceil_div64(len, n.chunk));
+    n.rows_per = inner == 1 ? kRowsPerSum : kColumnsPerSum;
+    n.blocks = ceil_div64(n.shape.rows, n.rows_per);
+    return n;
+}
+
+// Workspace: [partial sums of the rows' chunks][mean, rstd][partial sums of the parameters' gradients]
+struct NormWorkspace {
+    int64_t part = 0, stats = 0, params = 0, total = 0;
+    NormWorkspace(const Norm& n, size_t acc, bool backward) {
+        part = 0;
+        stats = part + align256(n.shape.rows * n.splits * 2 * acc);
+        params = stats + (backward ? 0 : align256(n.shape.rows * 2 * acc));
+        total = params + (backward ? align256(n.blocks * 2 * n.shape.len * acc) : 0);
+    }
+};
+
+size_t acc_bytes(int dtype) { return dtype == kF64 ? 8 : 4; }
+
+void check_norm(const char* name, int32_t dtype, int32_t param_dtype, const void* weight, const void* bias) {
+    SB_CHECK(dtype >= kF32 && dtype <= kBF16, name, ": unsupported dtype code ", dtype);
+    if (weight || bias)
+        SB_CHECK(param_dtype == dtype || (param_dtype == kF32 && dtype != kF64), name,
+                 ": weight and bias must be float32 or have the input's dtype");
+}
+
+template <typename T>
+void norm_forward(const char* name, const Norm& n, const void* x_, const void* weight, const void* bias, bool f32,
+                  double eps, void* y, void* mean_, void* rstd_, char* ws, cudaStream_t stream) {
+    using A = typename Storage<T>::acc;
+    const NormWorkspace w(n, sizeof(A), false);
+    const T* x = static_cast<const T*>(x_);
+    A* part = reinterpret_cast<A*>(ws + w.part);
+    A* mean = mean_ ? static_cast<A*>(mean_) : reinterpret_cast<A*>(ws + w.stats);
+    A* rstd = rstd_ ? static_cast<A*>(rstd_) : reinterpret_cast<A*>(ws + w.stats) + n.shape.rows;
+    const bool rows = n.shape.inner == 1;
+    const dim3 grid(grid_of(name, rows ? n.shape.rows : ceil_div64(n.shape.rows, 32)), n.splits);
+    const unsigned joins = grid_of(name, ceil_div64(n.shape.rows, kNormThreads));
+    auto stats = rows ? norm_stats_kernel<T, true> : norm_stats_kernel<T, false>;
+    auto apply = rows ? norm_apply_kernel<T, true> : norm_apply_kernel<T, false>;
+    stats<<<grid, kNormThreads, 0, stream>>>(x, part, n.shape, n.chunk);
+    SB_CUDA(cudaGetLastError());
+    norm_join_kernel<A><<<joins, kNormThreads, 0, stream>>>(part, mean, rstd, n.shape, n.chunk, n.splits, eps);
+    SB_CUDA(cudaGetLastError());
+    apply<<<grid, kNormThreads, 0, stream>>>(x, mean, rstd, weight, bias, f32, static_cast<T*>(y), n.shape, n.chunk);
+    SB_CUDA(cudaGetLastError());
+}
+
+template <typename T>
+void norm_backward(const char* name, const Norm& n, const void* gy_, const void* x_, const void* mean_,
+                   const void* rstd_, const void* weight, bool f32, const void* add, const DropRule& rule, void* dx,
+                   void* dropped, void* dw, void* db, char* ws, cudaStream_t stream) {
+    using A = typename Storage<T>::acc;
+    const NormWorkspace w(n, sizeof(A), true);
+    const T *gy = static_cast<const T*>(gy_), *x = static_cast<const T*>(x_);
+    const A *mean = static_cast<const A*>(mean_), *rstd = static_cast<const A*>(rstd_);
+    A* part = reinterpret_cast<A*>(ws + w.part);
+    A* sums = reinterpret_cast<A*>(ws + w.params);
+    const bool rows = n.shape.inner == 1;
+    if (dx || dropped) {
+        const dim3 grid(grid_of(name, rows ? n.shape.rows : ceil_div64(n.shape.rows, 32)), n.splits);
+        auto reduce = rows ? norm_bwd_sums_kernel<T, true> : norm_bwd_sums_kernel<T, false>;
+        auto apply = rows ? norm_bwd_apply_kernel<T, true> : norm_bwd_apply_kernel<T, false>;
+        reduce<<<grid, kNormThreads, 0, stream>>>(gy, x, mean, rstd, weight, f32, part, n.shape, n.chunk);
+        SB_CUDA(cudaGetLastError());
+        apply<<<grid, kNormThreads, 0, stream>>>(gy, x, mean, rstd, weight, f32, part, static_cast<const T*>(add),
+                                                 static_cast<T*>(dx), static_cast<T*>(dropped), rule, n.shape,
+                                                 n.chunk);
+        SB_CUDA(cudaGetLastError());
+    }
+    if (dw || db) {
+        if (rows) {
+            const int tiles = ceil_div(n.shape.len, kNormThreads);
+            norm_param_rows_kernel<T><<<grid_of(name, n.blocks * tiles), kNormThreads, 0, stream>>>(
+                gy, x, mean, rstd, sums, n.shape, n.rows_per, tiles);
+        } else {
+            norm_param_columns_kernel<T><<<grid_of(name, n.blocks * n.shape.len), kNormThreads, 0, stream>>>(
+                gy, x, mean, rstd, sums, n.shape, n.rows_per);
+        }
+        SB_CUDA(cudaGetLastError());
+        norm_param_final_kernel<T><<<ceil_div(n.shape.len, 32), kNormThreads, 0, stream>>>(sums, n.blocks, n.shape.len,
+                                                                                           dw, db, f32);
+        SB_CUDA(cudaGetLastError());
+    }
+}
+
+void check_workspace(const char* name, const void* workspace, int64_t have, int64_t need) {
+    if (have < need || (need > 0 && workspace == nullptr))
+        throw Failure{SERRON_ERR_WORKSPACE, concat(name, ": workspace of ", have, " bytes, ", need, " needed")};
+}
+
+// No rows: nothing to normalise, and gradients of the parameters that are sums of nothing.
+void zero_params(int len, int param_dtype, void* dw, void* db, cudaStream_t stream) {
+    if (dw) SB_CUDA(cudaMemsetAsync(dw, 0, len * elem_size(param_dtype), stream));
+    if (db) SB_CUDA(cudaMemsetAsync(db, 0, len * elem_size(param_dtype), stream));
+}
+
+int layer_norm_backward(const char* name, const void* grad_output, const void* grad_sum, const void* input,
+                        const void* mean, const void* rstd, int64_t outer, int64_t len, int64_t inner, int32_t dtype,
+                        const void* weight, int32_t param_dtype, double p, uint64_t seed, const void* seed_device,
+                        uint64_t sequence, void* grad_input, void* grad_dropped, void* grad_weight, void* grad_bias,
+                        void* workspace, int64_t workspace_bytes, int32_t device, void* stream_) {
+    return guarded([&] {
+        check_norm(name, dtype, param_dtype, grad_weight ? grad_weight : weight, grad_bias);
+        const Norm n = norm_of(name, outer, len, inner);
+        const DropRule rule = drop_rule(name, p, seed, seed_device, sequence);
+        const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+        if (n.numel() == 0) {
+            if (!grad_weight && !grad_bias) return;
+            DeviceScope scope(device);
+            return zero_params(n.shape.len, param_dtype, grad_weight, grad_bias, stream);
+        }
+        SB_CHECK(grad_output && input && mean && rstd, name, ": tensors must not be null");
+        check_workspace(name, workspace, workspace_bytes, NormWorkspace(n, acc_bytes(dtype), true).total);
+        DeviceScope scope(device);
+        with_type(dtype, [&](auto t) {
+            norm_backward<decltype(t)>(name, n, grad_output, input, mean, rstd, weight,
+                                       param_dtype == kF32 && dtype != kF32, grad_sum, rule, grad_input, grad_dropped,
+                                       grad_weight, grad_bias, static_cast<char*>(workspace), stream);
+        });
+    });
+}
+
+}  // namespace
+}  // namespace serron
+
+using namespace serron;
+
+extern "C" {
+
+int64_t serron_layer_norm_workspace_bytes(int64_t outer, int64_t len, int64_t inner, int32_t dtype, int32_t backward) {
+    int64_t bytes = -1;
+    const int rc = guarded([&] {
+        check_norm("serron::layer_norm", dtype, dtype, nullptr, nullptr);
+        bytes = NormWorkspace(norm_of("serron::layer_norm", outer, len, inner), acc_bytes(dtype), backward != 0).total;
+    });
+    return rc == SERRON_OK ? bytes : -1;
+}
+
+int serron_layer_norm(const void* input, int64_t outer, int64_t len, int64_t inner, int32_t dtype, const void* weight,
+                      const void* bias, int32_t param_dtype, double eps, void* output, void* mean, void* rstd,
+                      void* workspace, int64_t workspace_bytes, int32_t device, void* stream) {
+    const char* name = "serron::layer_norm";
+    return guarded([&] {
+        check_norm(name, dtype, param_dtype, weight, bias);
+        SB_CHECK(eps >= 0.0 && std::isfinite(eps), name, ": eps must be finite and not negative, got ", eps);
+        const Norm n = norm_of(name, outer, len, inner);
+        if (n.numel() == 0) return;
+        SB_CHECK(input && output, name, ": tensors must not be null");
+        check_workspace(name, workspace, workspace_bytes, NormWorkspace(n, acc_bytes(dtype), false).total);
+        DeviceScope scope(device);
+        with_type(dtype, [&](auto t) {
+            norm_forward<decltype(t)>(name, n, input, weight, bias, param_dtype == kF32 && dtype != kF32, eps, output,
+                                      mean, rstd, static_cast<char*>(workspace), static_cast<cudaStream_t>(stream));
+        });
+    });
+}
+
+int serron_layer_norm_backward(const void* grad_output, const void* input, const void* mean, const void* rstd,
+                               int64_t outer, int64_t len, int64_t inner, int32_t dtype, const void* weight,
+                               int32_t param_dtype, void* grad_input, void* grad_weight, void* grad_bias,
+                               void* workspace, int64_t workspace_bytes, int32_t device, void* stream) {
+    return layer_norm_backward("serron::layer_norm_backward", grad_output, nullptr, input, mean, rstd, outer, len,
+                               inner, dtype, weight, param_dtype, 0.0, 0, nullptr, 0, grad_input, nullptr, grad_weight,
+                               grad_bias, workspace, workspace_bytes, device, stream);
+}
+
+int serron_dropout(const void* input, const void* residual, int64_t numel, int64_t span, int32_t dtype, double p,
+                   uint64_t seed, const void* seed_device, uint64_t sequence, void* output, int32_t device,
+                   void* stream) {
+    const char* name = "serron::dropout";
+    return guarded([&] {
+        SB_CHECK(dtype >= kF32 && dtype <= kBF16, name, ": unsupported dtype code ", dtype);
+        SB_CHECK(numel >= 0, name, ": sizes must be non-negative");
+        SB_CHECK(span >= 1, name, ": a decision must cover at least one element, got ", span);
+        const DropRule rule = drop_rule(name, p, seed, seed_device, sequence);
+        if (numel == 0) return;
+        SB_CHECK(input && output, name, ": tensors must not be null");
+        DeviceScope scope(device);
+        with_type(dtype, [&](auto t) {
+            launch_dropout<decltype(t)>(name, input, residual, output, numel, span, rule,
+                                        static_cast<cudaStream_t>(stream));
+        });
+    });
+}
+
+int serron_dropout_add_layer_norm(const void* input, const void* residual, int64_t outer, int64_t len, int64_t inner,
+                                  int32_t dtype, const void* weight, const void* bias, int32_t param_dtype, double p,
+                                  uint64_t seed, const void* seed_device, uint64_t sequence, double eps, void* sum,
+                                  void* output, void* mean, void* rstd, void* workspace, int64_t workspace_bytes,
+                                  int32_t device, void* stream_) {
+    const char* name = "serron::dropout_add_layer_norm";
+    return guarded([&] {
+        check_norm(name, dtype, param_dtype, weight, bias);
+        SB_CHECK(eps >= 0.0 && std::isfinite(eps), name, ": eps must be finite and not negative, got ", eps);
+        const Norm n = norm_of(name, outer, len, inner);
+        const DropRule rule = drop_rule(name, p, seed, seed_device, sequence);
+        if (n.numel() == 0) return;
+        SB_CHECK(input && residual && sum && output, name, ": tensors must not be null");
+        check_workspace(name, workspace, workspace_bytes, NormWorkspace(n, acc_bytes(dtype), false).total);
+        const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+        DeviceScope scope(device);
+        with_type(dtype, [&](auto t) {
+            using T = decltype(t);
+            launch_dropout<T>(name, input, residual, sum, n.numel(), 1, rule, stream);
+            norm_forward<T>(name, n, sum, weight, bias, param_dtype == kF32 && dtype != kF32, eps, output, mean, rstd,
+                            static_cast<char*>(workspace), stream);
+        });
+    });
+}
+
+int serron_dropout_add_layer_norm_backward(const void* grad_output, const void* grad_sum, const void* sum,
+                                           const void* mean, const void* rstd, int64_t outer, int64_t len,
+                                           int64_t inner, int32_t dtype, const void* weight, int32_t param_dtype,
+                                           double p, uint64_t seed, const void* seed_device, uint64_t sequence,
+                                           void* grad_input, void* grad_residual, void* grad_weight, void* grad_bias,
+                                           void* workspace, int64_t workspace_bytes, int32_t device, void* stream) {
+    return layer_norm_backward("serron::dropout_add_layer_norm_backward", grad_output, grad_sum, sum, mean, rstd,
+                               outer, len, inner, dtype, weight, param_dtype, p, seed, seed_device, sequence,
+                               grad_residual, grad_input, grad_weight, grad_bias, workspace, workspace_bytes, device,
+                               stream);
+}
+
+}  // extern "C"

@@ -37,6 +37,14 @@ BORDER_TO_INT: dict[BorderMode, int] = {
 """Integer encoding of :class:`BorderMode` taken by the compiled operators."""
 
 
+class DropoutUnit(Enum):
+    """What :func:`serron_b200.functional.dropout` keeps or drops as a whole (no reference counterpart)."""
+
+    ELEMENT = "element"  #: every element by itself
+    CHANNEL = "channel"  #: the elements behind the first two dimensions: a feature map of an (N, C, H, W) input
+    SAMPLE = "sample"  #: the elements behind the first dimension: a residual branch of a sample
+
+
 class Algorithm(IntEnum):
     """Algorithm a compiled operator runs; ``AUTO`` lets the library choose, the others force one."""
 

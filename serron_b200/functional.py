@@ -6,16 +6,29 @@ Same functions, signatures, defaults and errors as packages/serron/torch-ext/ser
 in shared memory for the others) when the input and the structuring element share a dtype, autocast is
 off and the window is at most 7 a side; otherwise they are the reference's compositions.  Both give the
 same bits.  The reconstructions run on the library's fixed-point solver instead of a Python loop.
+
+``layer_norm``, ``dropout`` and ``dropout_add_layer_norm`` are what a network puts around the learnable
+layers; the reference has no counterpart.  They compute in float32 (float64 for float64 inputs) and return the
+input's dtype, so autocast leaves them as they are.  Their gradients cannot be differentiated again.
 """
 
 from __future__ import annotations
 
+import math
+
 import torch
 
-from . import _flatness, _ops
+from . import _flatness, _layer_ops, _ops
 from ._autotune import ensure_loaded
-from .autograd import _DerivedFunction, _DilateFunction, _ErodeFunction
-from .enums import BORDER_TO_INT, BorderMode
+from .autograd import (
+    _DerivedFunction,
+    _DilateFunction,
+    _DropoutAddLayerNormFunction,
+    _DropoutFunction,
+    _ErodeFunction,
+    _LayerNormFunction,
+)
+from .enums import BORDER_TO_INT, BorderMode, DropoutUnit
 
 
 def erosion(input_: torch.Tensor, kernel: torch.Tensor, *, border: BorderMode = BorderMode.REPLICATE) -> torch.Tensor:
@@ -131,3 +144,67 @@ def reconstruction_by_erosion(marker: torch.Tensor, mask: torch.Tensor, kernel: 
     """Fixed point of ``max(erosion(y), mask)`` from ``y = max(marker, mask)`` (the dual)."""
     return _reconstruct(marker, mask, kernel, border, dilate=False, max_iter=max_iter, check_every=check_every,
                         name="serron.reconstruction_by_erosion")
+
+
+def _records(*tensors: torch.Tensor | None) -> bool:
+    """Whether a backward pass can follow."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def layer_norm(input_: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
+               dim: int = 1, eps: float = 1e-5) -> torch.Tensor:
+    """``(input - mean) / sqrt(var + eps) * weight + bias`` with mean and (biased) variance over dimension ``dim``.
+
+    ``dim=1`` normalises the channels of an (N, C, H, W) map at every pixel, ``dim=-1`` the features of tokens.
+    ``weight`` and ``bias`` have one entry per element of ``dim``, in float32 or in the input's dtype; either may be
+    None.  Any dense memory order of ``input_`` (channels_last, a transposed view) is read and written as it lies.
+    """
+    _layer_ops.check_input("layer_norm", input_)
+    dim = _layer_ops.check_norm("layer_norm", input_, weight, bias, dim, eps)
+    if _records(input_, weight, bias):
+        return _LayerNormFunction.apply(input_, weight, bias, dim, eps)
+    return _layer_ops.layer_norm(input_, weight, bias, dim, eps, False)[0]
+
+
+def dropout(input_: torch.Tensor, p: float = 0.5, *, seed: int | torch.Tensor, sequence: int = 0,
+            unit: DropoutUnit = DropoutUnit.ELEMENT, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``input / (1 - p)`` where kept and 0 where dropped, each ``unit`` with probability ``p``; plus ``residual``.
+
+    The mask is never stored: decision j (in row-major order of the elements, channels or samples) keeps its unit when
+    word j % 4 of the Philox4x32-10 block with counter (j // 4, sequence) and key ``seed`` is at least
+    round(p * 2^32).  Calls with the same seed and sequence share their mask, so every call of a training step takes
+    a ``sequence`` (or a seed) of its own.  ``seed`` is an integer below 2^64, or an int64 CUDA tensor of one element,
+    which a captured CUDA graph reads anew at every replay.  A dropped unit is 0 whatever it held.
+    """
+    _layer_ops.check_input("dropout", input_)
+    p, seed, sequence = _layer_ops.check_drop("dropout", input_, p, seed, sequence)
+    if residual is not None:
+        _layer_ops.check_residual("dropout", input_, residual)
+    span = 1
+    if unit is not DropoutUnit.ELEMENT:
+        lead = 2 if DropoutUnit(unit) is DropoutUnit.CHANNEL else 1
+        if input_.dim() < lead:
+            raise ValueError(f"serron.dropout: unit {unit.value!r} needs an input of at least {lead} dimensions, got "
+                             f"{input_.dim()}")
+        span = max(1, math.prod(input_.shape[lead:]))
+    if _records(input_, residual):
+        return _DropoutFunction.apply(input_, residual, span, p, seed, sequence)
+    return _layer_ops.dropout(input_, residual, span, p, seed, sequence)
+
+
+def dropout_add_layer_norm(input_: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None,
+                           bias: torch.Tensor | None = None, *, p: float = 0.5, seed: int | torch.Tensor,
+                           sequence: int = 0, dim: int = 1, eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(y, h)`` with ``h = residual + dropout(input)`` and ``y = layer_norm(h, weight, bias)``, in one pass.
+
+    The end of a residual branch and the beginning of the next: ``h`` goes on along the residual path, ``y`` into the
+    next branch.  ``h`` is rounded to the input's dtype and normalised as it is returned.  Arguments as for
+    :func:`dropout` (by element) and :func:`layer_norm`; ``p=0`` (evaluation) needs no particular seed.
+    """
+    _layer_ops.check_input("dropout_add_layer_norm", input_)
+    p, seed, sequence = _layer_ops.check_drop("dropout_add_layer_norm", input_, p, seed, sequence)
+    _layer_ops.check_residual("dropout_add_layer_norm", input_, residual)
+    dim = _layer_ops.check_norm("dropout_add_layer_norm", input_, weight, bias, dim, eps)
+    if _records(input_, residual, weight, bias):
+        return _DropoutAddLayerNormFunction.apply(input_, residual, weight, bias, p, seed, sequence, dim, eps)
+    return _layer_ops.dropout_add_layer_norm(input_, residual, weight, bias, p, seed, sequence, dim, eps, False)[:2]
