@@ -251,17 +251,20 @@ __global__ void __launch_bounds__(kNormThreads)
     }
 }
 
-// 32 elements x 8 shares of the partial sums a block.
+// 32 elements x 32 shares of the partial sums a block.
+constexpr int kParamThreads = 1024;
 template <typename T>
-__global__ void __launch_bounds__(kNormThreads)
+__global__ void __launch_bounds__(kParamThreads)
     norm_param_final_kernel(const typename Storage<T>::acc* __restrict__ part, long long blocks, int len,
                             void* __restrict__ dw, void* __restrict__ db, bool f32) {
-    __shared__ double shared[2][8][32];
+    constexpr int kShares = kParamThreads / 32;
+    __shared__ double shared[2][kShares][33];
     const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
     const int l = blockIdx.x * 32 + lane;
     double w = 0.0, b = 0.0;
     if (l < len) {
-        for (long long k = share; k < blocks; k += 8) {
+#pragma unroll 8
+        for (long long k = share; k < blocks; k += kShares) {
             w += part[k * 2 * len + l];
             b += part[(k * 2 + 1) * len + l];
         }
@@ -269,13 +272,13 @@ __global__ void __launch_bounds__(kNormThreads)
     shared[0][share][lane] = w;
     shared[1][share][lane] = b;
     __syncthreads();
-    if (share != 0 || l >= len) return;
-    for (int k = 1; k < 8; ++k) {
-        w += shared[0][k][lane];
-        b += shared[1][k][lane];
+    // a warp joins the shares of one element of one gradient at a time
+    for (int i = share; i < 64; i += kShares) {
+        const double sum = warp_sum(shared[i >> 5][lane][i & 31]);
+        const int at = blockIdx.x * 32 + (i & 31);
+        void* out = i < 32 ? dw : db;
+        if (lane == 0 && at < len && out != nullptr) store_param<T>(out, at, f32, sum);
     }
-    if (dw) store_param<T>(dw, l, f32, w);
-    if (db) store_param<T>(db, l, f32, b);
 }
 
 }  // namespace serron

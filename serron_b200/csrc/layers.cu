@@ -9,8 +9,15 @@
 #include "dropout.cuh"
 #include "host_guard.h"
 #include "layer_norm.cuh"
+#include "layer_norm_fast.cuh"
+#include "layer_plan.h"
 
 namespace serron {
+
+// the register kernels, instantiated per storage type in layer_norm_<type>.cu
+template <typename T>
+cudaError_t norm_launch(const NormPlan& p, bool backward, bool join, const NormArgs<T>& args, cudaStream_t stream);
+
 namespace {
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
@@ -48,11 +55,40 @@ DropRule drop_rule(const char* name, double p, uint64_t seed, const void* seed_d
     return rule;
 }
 
+bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+constexpr int kDropVectors = 4;  // per thread
+
 template <typename T>
-void launch_dropout(const char* name, const void* x, const void* residual, void* y, int64_t n, int64_t span,
+void launch_dropout(const char* name, const void* x_, const void* residual_, void* y_, int64_t n, int64_t span,
                     const DropRule& rule, cudaStream_t stream) {
-    dropout_kernel<T><<<grid_of(name, ceil_div64(n, 256)), 256, 0, stream>>>(
-        static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<T*>(y), n, span, rule);
+    const T *x = static_cast<const T*>(x_), *residual = static_cast<const T*>(residual_);
+    T* y = static_cast<T*>(y_);
+    if constexpr (!std::is_same_v<T, double>) {
+        constexpr int V = 16 / sizeof(T), U = kDropVectors;
+        const bool wide = aligned(x, 16) && aligned(residual, 16) && aligned(y, 16);
+        if (span == 1 && wide) {
+            const unsigned blocks = grid_of(name, ceil_div64(n, 256 * U * V));
+            if (residual)
+                dropout_kernel<T, V, U, true><<<blocks, 256, 0, stream>>>(x, residual, y, n, rule);
+            else
+                dropout_kernel<T, V, U, false><<<blocks, 256, 0, stream>>>(x, residual, y, n, rule);
+            SB_CUDA(cudaGetLastError());
+            return;
+        }
+        if (span >= 256 && n % span == 0) {
+            const int64_t width = wide && span % V == 0 ? V : 1;
+            const int64_t pieces = ceil_div64(span, 256 * U * width);
+            const unsigned blocks = grid_of(name, n / span * pieces);
+            if (width > 1)
+                dropout_units_kernel<T, V, U><<<blocks, 256, 0, stream>>>(x, residual, y, span, pieces, rule);
+            else
+                dropout_units_kernel<T, 1, U><<<blocks, 256, 0, stream>>>(x, residual, y, span, pieces, rule);
+            SB_CUDA(cudaGetLastError());
+            return;
+        }
+    }
+    dropout_any_kernel<T><<<grid_of(name, ceil_div64(n, 256)), 256, 0, stream>>>(x, residual, y, n, span, rule);
     SB_CUDA(cudaGetLastError());
 }
 
@@ -65,6 +101,20 @@ struct Norm {
     int rows_per = 0;           // rows a partial sum of the parameters' gradients covers
     int64_t blocks = 0;         // such sums
     int64_t numel() const { return shape.rows * shape.len; }
+    int64_t inner = 1;
+
+    // The plan of the widest vectors that the sizes and `fits` (the pointers) allow; not ok where no register kernel
+    // takes the call.
+    template <typename F>
+    NormPlan plan(int dtype, bool backward, F&& fits) const {
+        for (const int* v = plan_widths(inner == 1, static_cast<int>(elem_size(dtype))); dtype != kF64 && *v; ++v) {
+            if (!fits(*v)) continue;
+            const NormPlan p =
+                norm_plan(shape.rows, shape.len, inner, *v, static_cast<int>(elem_size(dtype)), backward);
+            if (p.ok) return p;
+        }
+        return NormPlan();
+    }
 };
 
 // Rows per first-level sum of the parameters' gradients: at most 128 additions in a row (32 per thread where a
@@ -82,6 +132,7 @@ Norm norm_of(const char* name, int64_t outer, int64_t len, int64_t inner) {
     n.shape.rows = outer * inner;
     n.shape.len = static_cast<int>(len);
     n.shape.inner = static_cast<int>(std::max<int64_t>(inner, 1));
+    n.inner = n.shape.inner;
     n.chunk = static_cast<int>(std::max<int64_t>(inner == 1 ? 8192 : 1024, ceil_div64(len, 65535)));
     n.splits = static_cast<int>(ceil_div64(len, n.chunk));
     n.rows_per = inner == 1 ? kRowsPerSum : kColumnsPerSum;
@@ -89,7 +140,8 @@ Norm norm_of(const char* name, int64_t outer, int64_t len, int64_t inner) {
     return n;
 }
 
-// Workspace: [partial sums of the rows' chunks][mean, rstd][partial sums of the parameters' gradients]
+// Workspace of the kernels for any length: [partial sums of the rows' chunks][mean, rstd][partial sums of the
+// parameters' gradients]; of the register kernels: the last part alone.
 struct NormWorkspace {
     int64_t part = 0, stats = 0, params = 0, total = 0;
     NormWorkspace(const Norm& n, size_t acc, bool backward) {
@@ -100,7 +152,18 @@ struct NormWorkspace {
     }
 };
 
-size_t acc_bytes(int dtype) { return dtype == kF64 ? 8 : 4; }
+// What a call may need, whatever its pointers' alignment.
+int64_t workspace_bytes_of(const Norm& n, int dtype, bool backward) {
+    const size_t acc = dtype == kF64 ? 8 : 4;
+    bool any = false;  // whether some alignment leaves the call to the kernels for any length
+    int64_t bytes = 0;
+    for (int width = 1; width <= 8; width *= 2) {
+        const NormPlan p = n.plan(dtype, backward, [&](int v) { return v <= width; });
+        any = any || !p.ok;
+        if (p.ok && backward) bytes = std::max(bytes, align256(p.blocks * 2 * n.shape.len * int64_t(sizeof(float))));
+    }
+    return n.numel() == 0 ? 0 : any ? std::max(bytes, NormWorkspace(n, acc, backward).total) : bytes;
+}
 
 void check_norm(const char* name, int32_t dtype, int32_t param_dtype, const void* weight, const void* bias) {
     SB_CHECK(dtype >= kF32 && dtype <= kBF16, name, ": unsupported dtype code ", dtype);
@@ -110,9 +173,62 @@ void check_norm(const char* name, int32_t dtype, int32_t param_dtype, const void
 }
 
 template <typename T>
+constexpr int dtype_of = std::is_same_v<T, float>    ? kF32
+                         : std::is_same_v<T, __half> ? kF16
+                         : std::is_same_v<T, double> ? kF64
+                                                     : kBF16;
+
+// Every pointer on a boundary of `bytes` (null ones are).
+template <typename... P>
+bool fits(size_t bytes, P... pointers) {
+    return (aligned(pointers, bytes) && ...);
+}
+// Parameters are read V at a time in their own type, float32 ones at most four at a time.
+template <typename T, typename... P>
+bool params_fit(int V, bool f32, P... pointers) {
+    return fits(f32 ? (V >= 4 ? 16 : 4) : V * sizeof(T), pointers...);
+}
+
+template <typename T>
+void param_final(const typename Storage<T>::acc* sums, int64_t blocks, int len, void* dw, void* db, bool f32,
+                 cudaStream_t stream) {
+    norm_param_final_kernel<T><<<ceil_div(len, 32), kParamThreads, 0, stream>>>(sums, blocks, len, dw, db, f32);
+    SB_CUDA(cudaGetLastError());
+}
+
+template <typename T>
 void norm_forward(const char* name, const Norm& n, const void* x_, const void* weight, const void* bias, bool f32,
-                  double eps, void* y, void* mean_, void* rstd_, char* ws, cudaStream_t stream) {
+                  double eps, void* y, void* mean_, void* rstd_, char* ws, cudaStream_t stream,
+                  const void* residual, void* sum, const DropRule& rule) {
     using A = typename Storage<T>::acc;
+    const bool join = residual != nullptr;
+    if constexpr (!std::is_same_v<T, double>) {
+        const NormPlan p = n.plan(dtype_of<T>, false, [&](int v) {
+            return fits(v * sizeof(T), x_, residual, sum, y) && params_fit<T>(v, f32, weight, bias);
+        });
+        if (p.ok) {
+            NormArgs<T> a;
+            a.x = static_cast<const T*>(x_);
+            a.residual = static_cast<const T*>(residual);
+            a.weight = weight;
+            a.bias = bias;
+            a.f32 = f32;
+            a.sum = static_cast<T*>(sum);
+            a.y = static_cast<T*>(y);
+            a.mean = static_cast<float*>(mean_);
+            a.rstd = static_cast<float*>(rstd_);
+            a.eps = static_cast<float>(eps);
+            a.shape = n.shape;
+            a.rule = rule;
+            a.tiles = p.tiles;
+            SB_CUDA(norm_launch<T>(p, false, join, a, stream));
+            return;
+        }
+    }
+    if (join) {
+        launch_dropout<T>(name, x_, residual, sum, n.numel(), 1, rule, stream);
+        x_ = sum;
+    }
     const NormWorkspace w(n, sizeof(A), false);
     const T* x = static_cast<const T*>(x_);
     A* part = reinterpret_cast<A*>(ws + w.part);
@@ -134,8 +250,32 @@ void norm_forward(const char* name, const Norm& n, const void* x_, const void* w
 template <typename T>
 void norm_backward(const char* name, const Norm& n, const void* gy_, const void* x_, const void* mean_,
                    const void* rstd_, const void* weight, bool f32, const void* add, const DropRule& rule, void* dx,
-                   void* dropped, void* dw, void* db, char* ws, cudaStream_t stream) {
+                   void* dropped, void* dw, void* db, char* ws, cudaStream_t stream, bool join) {
     using A = typename Storage<T>::acc;
+    if constexpr (!std::is_same_v<T, double>) {
+        const NormPlan p = n.plan(dtype_of<T>, true, [&](int v) {
+            return fits(v * sizeof(T), gy_, x_, add, dx, dropped) && params_fit<T>(v, f32, weight);
+        });
+        if (p.ok) {
+            NormArgs<T> a;
+            a.x = static_cast<const T*>(x_);
+            a.weight = weight;
+            a.f32 = f32;
+            a.mean = static_cast<float*>(const_cast<void*>(mean_));
+            a.rstd = static_cast<float*>(const_cast<void*>(rstd_));
+            a.gy = static_cast<const T*>(gy_);
+            a.add = static_cast<const T*>(add);
+            a.dx = static_cast<T*>(dx);
+            a.dropped = static_cast<T*>(dropped);
+            a.part = dw || db ? reinterpret_cast<float*>(ws) : nullptr;
+            a.shape = n.shape;
+            a.rule = rule;
+            a.tiles = p.tiles;
+            SB_CUDA(norm_launch<T>(p, true, join, a, stream));
+            if (dw || db) param_final<T>(a.part, p.blocks, n.shape.len, dw, db, f32, stream);
+            return;
+        }
+    }
     const NormWorkspace w(n, sizeof(A), true);
     const T *gy = static_cast<const T*>(gy_), *x = static_cast<const T*>(x_);
     const A *mean = static_cast<const A*>(mean_), *rstd = static_cast<const A*>(rstd_);
@@ -163,9 +303,7 @@ void norm_backward(const char* name, const Norm& n, const void* gy_, const void*
                 gy, x, mean, rstd, sums, n.shape, n.rows_per);
         }
         SB_CUDA(cudaGetLastError());
-        norm_param_final_kernel<T><<<ceil_div(n.shape.len, 32), kNormThreads, 0, stream>>>(sums, n.blocks, n.shape.len,
-                                                                                           dw, db, f32);
-        SB_CUDA(cudaGetLastError());
+        param_final<T>(sums, n.blocks, n.shape.len, dw, db, f32, stream);
     }
 }
 
@@ -180,7 +318,7 @@ void zero_params(int len, int param_dtype, void* dw, void* db, cudaStream_t stre
     if (db) SB_CUDA(cudaMemsetAsync(db, 0, len * elem_size(param_dtype), stream));
 }
 
-int layer_norm_backward(const char* name, const void* grad_output, const void* grad_sum, const void* input,
+int layer_norm_backward(const char* name, bool join, const void* grad_output, const void* grad_sum, const void* input,
                         const void* mean, const void* rstd, int64_t outer, int64_t len, int64_t inner, int32_t dtype,
                         const void* weight, int32_t param_dtype, double p, uint64_t seed, const void* seed_device,
                         uint64_t sequence, void* grad_input, void* grad_dropped, void* grad_weight, void* grad_bias,
@@ -196,12 +334,12 @@ int layer_norm_backward(const char* name, const void* grad_output, const void* g
             return zero_params(n.shape.len, param_dtype, grad_weight, grad_bias, stream);
         }
         SB_CHECK(grad_output && input && mean && rstd, name, ": tensors must not be null");
-        check_workspace(name, workspace, workspace_bytes, NormWorkspace(n, acc_bytes(dtype), true).total);
+        check_workspace(name, workspace, workspace_bytes, workspace_bytes_of(n, dtype, true));
         DeviceScope scope(device);
         with_type(dtype, [&](auto t) {
             norm_backward<decltype(t)>(name, n, grad_output, input, mean, rstd, weight,
                                        param_dtype == kF32 && dtype != kF32, grad_sum, rule, grad_input, grad_dropped,
-                                       grad_weight, grad_bias, static_cast<char*>(workspace), stream);
+                                       grad_weight, grad_bias, static_cast<char*>(workspace), stream, join);
         });
     });
 }
@@ -217,7 +355,7 @@ int64_t serron_layer_norm_workspace_bytes(int64_t outer, int64_t len, int64_t in
     int64_t bytes = -1;
     const int rc = guarded([&] {
         check_norm("serron::layer_norm", dtype, dtype, nullptr, nullptr);
-        bytes = NormWorkspace(norm_of("serron::layer_norm", outer, len, inner), acc_bytes(dtype), backward != 0).total;
+        bytes = workspace_bytes_of(norm_of("serron::layer_norm", outer, len, inner), dtype, backward != 0);
     });
     return rc == SERRON_OK ? bytes : -1;
 }
@@ -232,11 +370,12 @@ int serron_layer_norm(const void* input, int64_t outer, int64_t len, int64_t inn
         const Norm n = norm_of(name, outer, len, inner);
         if (n.numel() == 0) return;
         SB_CHECK(input && output, name, ": tensors must not be null");
-        check_workspace(name, workspace, workspace_bytes, NormWorkspace(n, acc_bytes(dtype), false).total);
+        check_workspace(name, workspace, workspace_bytes, workspace_bytes_of(n, dtype, false));
         DeviceScope scope(device);
         with_type(dtype, [&](auto t) {
             norm_forward<decltype(t)>(name, n, input, weight, bias, param_dtype == kF32 && dtype != kF32, eps, output,
-                                      mean, rstd, static_cast<char*>(workspace), static_cast<cudaStream_t>(stream));
+                                      mean, rstd, static_cast<char*>(workspace), static_cast<cudaStream_t>(stream),
+                                      nullptr, nullptr, DropRule());
         });
     });
 }
@@ -245,7 +384,7 @@ int serron_layer_norm_backward(const void* grad_output, const void* input, const
                                int64_t outer, int64_t len, int64_t inner, int32_t dtype, const void* weight,
                                int32_t param_dtype, void* grad_input, void* grad_weight, void* grad_bias,
                                void* workspace, int64_t workspace_bytes, int32_t device, void* stream) {
-    return layer_norm_backward("serron::layer_norm_backward", grad_output, nullptr, input, mean, rstd, outer, len,
+    return layer_norm_backward("serron::layer_norm_backward", false, grad_output, nullptr, input, mean, rstd, outer, len,
                                inner, dtype, weight, param_dtype, 0.0, 0, nullptr, 0, grad_input, nullptr, grad_weight,
                                grad_bias, workspace, workspace_bytes, device, stream);
 }
@@ -282,14 +421,13 @@ int serron_dropout_add_layer_norm(const void* input, const void* residual, int64
         const DropRule rule = drop_rule(name, p, seed, seed_device, sequence);
         if (n.numel() == 0) return;
         SB_CHECK(input && residual && sum && output, name, ": tensors must not be null");
-        check_workspace(name, workspace, workspace_bytes, NormWorkspace(n, acc_bytes(dtype), false).total);
+        check_workspace(name, workspace, workspace_bytes, workspace_bytes_of(n, dtype, false));
         const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
         DeviceScope scope(device);
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
-            launch_dropout<T>(name, input, residual, sum, n.numel(), 1, rule, stream);
-            norm_forward<T>(name, n, sum, weight, bias, param_dtype == kF32 && dtype != kF32, eps, output, mean, rstd,
-                            static_cast<char*>(workspace), stream);
+            norm_forward<T>(name, n, input, weight, bias, param_dtype == kF32 && dtype != kF32, eps, output, mean, rstd,
+                            static_cast<char*>(workspace), stream, residual, sum, rule);
         });
     });
 }
@@ -300,7 +438,7 @@ int serron_dropout_add_layer_norm_backward(const void* grad_output, const void* 
                                            double p, uint64_t seed, const void* seed_device, uint64_t sequence,
                                            void* grad_input, void* grad_residual, void* grad_weight, void* grad_bias,
                                            void* workspace, int64_t workspace_bytes, int32_t device, void* stream) {
-    return layer_norm_backward("serron::dropout_add_layer_norm_backward", grad_output, grad_sum, sum, mean, rstd,
+    return layer_norm_backward("serron::dropout_add_layer_norm_backward", true, grad_output, grad_sum, sum, mean, rstd,
                                outer, len, inner, dtype, weight, param_dtype, p, seed, seed_device, sequence,
                                grad_residual, grad_input, grad_weight, grad_bias, workspace, workspace_bytes, device,
                                stream);
