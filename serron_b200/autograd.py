@@ -13,16 +13,13 @@ the same pass (so the promoted copy of the input is never made); other autocast 
 and the backward searches the windows itself.  After the autocast forward the backward reads the float16
 ``grad_output`` and writes ``grad_input`` in the input's dtype directly (float32 sums in between), which
 gives the values of the reference's casts up and down without making the copies.
-
-The layer operators at the end (layer norm, dropout and their join) have no reference counterpart.
 """
 
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import _flatness, _layer_ops, _lib, _ops
+from . import _flatness, _lib, _ops
 from ._autotune import ensure_loaded, select_algorithm
 from ._ops import add_op_namespace_prefix, ops
 from .enums import Algorithm
@@ -176,82 +173,3 @@ class _DerivedFunction(torch.autograd.Function):
             else:
                 grad_input, grad_kernel = g_1, k_2 + k_1
         return (grad_input if needs_input else None), (grad_kernel if needs_kernel else None), None, None
-
-
-# ------------------------------------------------------------------------------------------------
-# layer operators: statistics (layer norm) or nothing but the seed (dropout) are kept between the passes
-# ------------------------------------------------------------------------------------------------
-def _param_dtype(*params: torch.Tensor | None) -> torch.dtype | None:
-    return next((p.dtype for p in params if p is not None), None)
-
-
-class _LayerNormFunction(torch.autograd.Function):
-    """``serron_layer_norm`` and its backward, for arguments that are already checked."""
-
-    @staticmethod
-    def forward(ctx, input_: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, dim: int,
-                eps: float):
-        y, x, mean, rstd = _layer_ops.layer_norm(input_, weight, bias, dim, eps, True)
-        ctx.save_for_backward(x, mean, rstd, weight)
-        ctx.dim = dim
-        ctx.param_dtype = _param_dtype(weight, bias) or x.dtype
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output: torch.Tensor):
-        x, mean, rstd, weight = ctx.saved_tensors
-        return (*_layer_ops.layer_norm_backward(grad_output, x, mean, rstd, weight, ctx.param_dtype, ctx.dim,
-                                                ctx.needs_input_grad[:3]), None, None)
-
-
-class _DropoutFunction(torch.autograd.Function):
-    """``serron_dropout``; the backward draws the same mask again."""
-
-    @staticmethod
-    def forward(ctx, input_: torch.Tensor, residual: torch.Tensor | None, span: int, p: float,
-                seed: int | torch.Tensor, sequence: int):
-        ctx.save_for_backward(seed if isinstance(seed, torch.Tensor) else None)
-        ctx.rule = (span, p, seed if isinstance(seed, int) else None, sequence)
-        return _layer_ops.dropout(input_, residual, span, p, seed, sequence)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output: torch.Tensor):
-        span, p, seed, sequence = ctx.rule
-        (seed_tensor,) = ctx.saved_tensors
-        grad_input = None
-        if ctx.needs_input_grad[0]:
-            grad_input = _layer_ops.dropout(grad_output, None, span, p, seed if seed_tensor is None else seed_tensor,
-                                            sequence)
-        return grad_input, (grad_output if ctx.needs_input_grad[1] else None), None, None, None, None
-
-
-class _DropoutAddLayerNormFunction(torch.autograd.Function):
-    """``serron_dropout_add_layer_norm`` and its backward, for arguments that are already checked."""
-
-    @staticmethod
-    def forward(ctx, input_: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None,
-                bias: torch.Tensor | None, p: float, seed: int | torch.Tensor, sequence: int, dim: int, eps: float):
-        y, h, mean, rstd = _layer_ops.dropout_add_layer_norm(input_, residual, weight, bias, p, seed, sequence, dim,
-                                                             eps, True)
-        ctx.save_for_backward(h, mean, rstd, weight, seed if isinstance(seed, torch.Tensor) else None)
-        ctx.set_materialize_grads(False)
-        ctx.rule = (p, seed if isinstance(seed, int) else None, sequence)
-        ctx.dim = dim
-        ctx.param_dtype = _param_dtype(weight, bias) or h.dtype
-        return y, h
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output: torch.Tensor | None, grad_sum: torch.Tensor | None):
-        h, mean, rstd, weight, seed_tensor = ctx.saved_tensors
-        p, seed, sequence = ctx.rule
-        if grad_output is None:
-            if grad_sum is None:
-                return (None,) * 9
-            grad_output = torch.zeros_like(h)
-        grads = _layer_ops.dropout_add_layer_norm_backward(
-            grad_output, grad_sum, h, mean, rstd, weight, ctx.param_dtype, p, seed if seed_tensor is None else seed_tensor,
-            sequence, ctx.dim, ctx.needs_input_grad[:4])
-        return (*grads, None, None, None, None, None)

@@ -20,14 +20,7 @@ import torch
 
 from . import _flatness, _layer_ops, _ops
 from ._autotune import ensure_loaded
-from .autograd import (
-    _DerivedFunction,
-    _DilateFunction,
-    _DropoutAddLayerNormFunction,
-    _DropoutFunction,
-    _ErodeFunction,
-    _LayerNormFunction,
-)
+from .autograd import _DerivedFunction, _DilateFunction, _ErodeFunction
 from .enums import BORDER_TO_INT, BorderMode, DropoutUnit
 
 
@@ -146,11 +139,6 @@ def reconstruction_by_erosion(marker: torch.Tensor, mask: torch.Tensor, kernel: 
                         name="serron.reconstruction_by_erosion")
 
 
-def _records(*tensors: torch.Tensor | None) -> bool:
-    """Whether a backward pass can follow."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
 def layer_norm(input_: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
                dim: int = 1, eps: float = 1e-5) -> torch.Tensor:
     """``(input - mean) / sqrt(var + eps) * weight + bias`` with mean and (biased) variance over dimension ``dim``.
@@ -161,9 +149,7 @@ def layer_norm(input_: torch.Tensor, weight: torch.Tensor | None = None, bias: t
     """
     _layer_ops.check_input("layer_norm", input_)
     dim = _layer_ops.check_norm("layer_norm", input_, weight, bias, dim, eps)
-    if _records(input_, weight, bias):
-        return _LayerNormFunction.apply(input_, weight, bias, dim, eps)
-    return _layer_ops.layer_norm(input_, weight, bias, dim, eps, False)[0]
+    return _layer_ops.binding().layer_norm(input_, weight, bias, dim, eps)
 
 
 def dropout(input_: torch.Tensor, p: float = 0.5, *, seed: int | torch.Tensor, sequence: int = 0,
@@ -177,7 +163,7 @@ def dropout(input_: torch.Tensor, p: float = 0.5, *, seed: int | torch.Tensor, s
     which a captured CUDA graph reads anew at every replay.  A dropped unit is 0 whatever it held.
     """
     _layer_ops.check_input("dropout", input_)
-    p, seed, sequence = _layer_ops.check_drop("dropout", input_, p, seed, sequence)
+    rule = _layer_ops.check_drop("dropout", input_, p, seed, sequence)
     if residual is not None:
         _layer_ops.check_residual("dropout", input_, residual)
     span = 1
@@ -187,9 +173,7 @@ def dropout(input_: torch.Tensor, p: float = 0.5, *, seed: int | torch.Tensor, s
             raise ValueError(f"serron.dropout: unit {unit.value!r} needs an input of at least {lead} dimensions, got "
                              f"{input_.dim()}")
         span = max(1, math.prod(input_.shape[lead:]))
-    if _records(input_, residual):
-        return _DropoutFunction.apply(input_, residual, span, p, seed, sequence)
-    return _layer_ops.dropout(input_, residual, span, p, seed, sequence)
+    return _layer_ops.binding().dropout(input_, residual, span, *rule)
 
 
 def dropout_add_layer_norm(input_: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None,
@@ -202,9 +186,7 @@ def dropout_add_layer_norm(input_: torch.Tensor, residual: torch.Tensor, weight:
     :func:`dropout` (by element) and :func:`layer_norm`; ``p=0`` (evaluation) needs no particular seed.
     """
     _layer_ops.check_input("dropout_add_layer_norm", input_)
-    p, seed, sequence = _layer_ops.check_drop("dropout_add_layer_norm", input_, p, seed, sequence)
+    rule = _layer_ops.check_drop("dropout_add_layer_norm", input_, p, seed, sequence)
     _layer_ops.check_residual("dropout_add_layer_norm", input_, residual)
     dim = _layer_ops.check_norm("dropout_add_layer_norm", input_, weight, bias, dim, eps)
-    if _records(input_, residual, weight, bias):
-        return _DropoutAddLayerNormFunction.apply(input_, residual, weight, bias, p, seed, sequence, dim, eps)
-    return _layer_ops.dropout_add_layer_norm(input_, residual, weight, bias, p, seed, sequence, dim, eps, False)[:2]
+    return _layer_ops.binding().dropout_add_layer_norm(input_, residual, weight, bias, *rule, dim, eps)
