@@ -13,22 +13,40 @@ namespace serron {
 // of two 32 x 32 -> 64 bit products over a counter, under a key that grows by a constant a round.  Block j of
 // sequence q under seed s is the cipher of counter (j, q) with key s, all 64 bits wide, low word first.
 // ------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint4 philox(uint64_t block, uint64_t sequence, uint64_t seed) {
-    uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32);
+constexpr int kPhiloxRounds = 10;
+constexpr uint32_t kPhiloxMul0 = 0xD2511F53u, kPhiloxMul1 = 0xCD9E8D57u;
+constexpr uint32_t kPhiloxKey0 = 0x9E3779B9u, kPhiloxKey1 = 0xBB67AE85u;
+
+// The keys of all rounds.
+struct PhiloxKeys {
+    uint32_t k0[kPhiloxRounds], k1[kPhiloxRounds];
+
+    __host__ __device__ __forceinline__ void set(uint64_t seed) {
+        for (int r = 0; r < kPhiloxRounds; ++r) {
+            k0[r] = static_cast<uint32_t>(seed) + r * kPhiloxKey0;
+            k1[r] = static_cast<uint32_t>(seed >> 32) + r * kPhiloxKey1;
+        }
+    }
+};
+
+// The words of block (low, high).  Where `high` and `sequence` are the same for all threads, so is half of the first two
+// rounds, and the compiler computes it once.
+__device__ __forceinline__ uint4 philox(uint32_t low, uint32_t high, uint64_t sequence, const PhiloxKeys& keys) {
+    uint32_t c0 = low, c1 = high;
     uint32_t c2 = static_cast<uint32_t>(sequence), c3 = static_cast<uint32_t>(sequence >> 32);
-    uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
 #pragma unroll
-    for (int round = 0; round < 10; ++round) {
-        const uint64_t a = static_cast<uint64_t>(c0) * 0xD2511F53u;
-        const uint64_t b = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
-        c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
+    for (int r = 0; r < kPhiloxRounds; ++r) {
+        const uint64_t a = static_cast<uint64_t>(c0) * kPhiloxMul0;
+        const uint64_t b = static_cast<uint64_t>(c2) * kPhiloxMul1;
+        c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ keys.k0[r];
         c1 = static_cast<uint32_t>(b);
-        c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
+        c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ keys.k1[r];
         c3 = static_cast<uint32_t>(a);
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
     }
     return make_uint4(c0, c1, c2, c3);
+}
+__device__ __forceinline__ uint4 philox(long long block, uint64_t sequence, const PhiloxKeys& keys) {
+    return philox(static_cast<uint32_t>(block), static_cast<uint32_t>(block >> 32), sequence, keys);
 }
 
 __device__ __forceinline__ uint32_t word_of(const uint4& block, int i) {
@@ -37,15 +55,19 @@ __device__ __forceinline__ uint32_t word_of(const uint4& block, int i) {
 
 // The dropout rule: decision j keeps its elements when word j % 4 of block j / 4 is at least `threshold`.
 struct DropRule {
-    uint64_t seed = 0;
-    const uint64_t* seed_device = nullptr;  // read by the kernel in place of `seed` where set
+    PhiloxKeys keys;                        // of the seed, unless it is in device memory
+    const uint64_t* seed_device = nullptr;  // read by the kernel in place of `keys` where set
     uint64_t sequence = 0;
     uint32_t threshold = 0;  // round(p * 2^32)
-    int all = 0;             // p rounds to one: every element is dropped
+    bool all = false;        // p rounds to one: every element is dropped
     double scale = 1.0;      // 1 / (1 - p)
 
-    __device__ __forceinline__ uint64_t key() const { return seed_device ? __ldg(seed_device) : seed; }
-    __device__ __forceinline__ bool keeps(uint32_t word) const { return word >= threshold && !all; }
+    // the keys wherever the seed is (in registers)
+    __device__ __forceinline__ PhiloxKeys own_keys() const {
+        PhiloxKeys k = keys;
+        if (seed_device) k.set(__ldg(seed_device));
+        return k;
+    }
 };
 
 // A kept element, scaled; a dropped one is zero whatever it held (NaN and infinities too).  The product is rounded

@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(kNormThreads)
         if (add) v += S::load(add[e]);
         if (dx) dx[e] = S::store(v);
         if (dropped) {
-            const bool kept = rule.keeps(word_of(philox(e >> 2, rule.sequence, rule.key()), e & 3));
+            const bool kept =
+                word_of(philox(e >> 2, rule.sequence, rule.own_keys()), e & 3) >= rule.threshold && !rule.all;
             dropped[e] = S::store(kept ? scaled<A>(v, A(rule.scale)) : A(0));
         }
     }
@@ -251,33 +252,29 @@ __global__ void __launch_bounds__(kNormThreads)
     }
 }
 
-// 32 elements x 32 shares of the partial sums a block.
+// Each block: 32 of the 2 * len columns (dw, then db), blockDim.x / 32 shares of the partial sums.
 constexpr int kParamThreads = 1024;
 template <typename T>
 __global__ void __launch_bounds__(kParamThreads)
-    norm_param_final_kernel(const typename Storage<T>::acc* __restrict__ part, long long blocks, int len,
+    norm_param_final_kernel(const typename Storage<T>::acc* __restrict__ part, int blocks, int len,
                             void* __restrict__ dw, void* __restrict__ db, bool f32) {
-    constexpr int kShares = kParamThreads / 32;
-    __shared__ double shared[2][kShares][33];
-    const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
-    const int l = blockIdx.x * 32 + lane;
-    double w = 0.0, b = 0.0;
-    if (l < len) {
+    __shared__ double shared[kParamThreads / 32][33];
+    const int lane = threadIdx.x & 31, share = threadIdx.x >> 5, shares = blockDim.x >> 5;
+    const long long width = 2ll * len, column = blockIdx.x * 32ll + lane;
+    double sum = 0.0;
+    if (column < width) {
+        const typename Storage<T>::acc* p = part + column;
 #pragma unroll 8
-        for (long long k = share; k < blocks; k += kShares) {
-            w += part[k * 2 * len + l];
-            b += part[(k * 2 + 1) * len + l];
-        }
+        for (int k = share; k < blocks; k += shares) sum += p[k * width];
     }
-    shared[0][share][lane] = w;
-    shared[1][share][lane] = b;
+    shared[share][lane] = sum;
     __syncthreads();
-    // a warp joins the shares of one element of one gradient at a time
-    for (int i = share; i < 64; i += kShares) {
-        const double sum = warp_sum(shared[i >> 5][lane][i & 31]);
-        const int at = blockIdx.x * 32 + (i & 31);
-        void* out = i < 32 ? dw : db;
-        if (lane == 0 && at < len && out != nullptr) store_param<T>(out, at, f32, sum);
+    // a warp joins the shares of one column at a time
+    for (int i = share; i < 32; i += shares) {
+        const double total = warp_sum(lane < shares ? shared[lane][i] : 0.0);
+        const long long c = blockIdx.x * 32ll + i;
+        void* out = c < len ? dw : db;
+        if (lane == 0 && c < width && out != nullptr) store_param<T>(out, c < len ? c : c - len, f32, total);
     }
 }
 

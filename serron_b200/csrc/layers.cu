@@ -45,7 +45,7 @@ unsigned grid_of(const char* name, int64_t blocks) {
 DropRule drop_rule(const char* name, double p, uint64_t seed, const void* seed_device, uint64_t sequence) {
     SB_CHECK(p >= 0.0 && p <= 1.0, name, ": p must be between 0 and 1, got ", p);
     DropRule rule;
-    rule.seed = seed;
+    rule.keys.set(seed);
     rule.seed_device = static_cast<const uint64_t*>(seed_device);
     rule.sequence = sequence;
     const double threshold = std::nearbyint(p * 4294967296.0);
@@ -67,12 +67,13 @@ void launch_dropout(const char* name, const void* x_, const void* residual_, voi
     if constexpr (!std::is_same_v<T, double>) {
         constexpr int V = 16 / sizeof(T), U = kDropVectors;
         const bool wide = aligned(x, 16) && aligned(residual, 16) && aligned(y, 16);
+        if (rule.all) span = n;  // one decision for everything
         if (span == 1 && wide) {
             const unsigned blocks = grid_of(name, ceil_div64(n, 256 * U * V));
-            if (residual)
-                dropout_kernel<T, V, U, true><<<blocks, 256, 0, stream>>>(x, residual, y, n, rule);
-            else
-                dropout_kernel<T, V, U, false><<<blocks, 256, 0, stream>>>(x, residual, y, n, rule);
+            auto kernel = rule.seed_device
+                              ? (residual ? dropout_kernel<T, V, U, true, true> : dropout_kernel<T, V, U, false, true>)
+                              : (residual ? dropout_kernel<T, V, U, true, false> : dropout_kernel<T, V, U, false, false>);
+            kernel<<<blocks, 256, 0, stream>>>(x, residual, y, n, rule);
             SB_CUDA(cudaGetLastError());
             return;
         }
@@ -192,7 +193,11 @@ bool params_fit(int V, bool f32, P... pointers) {
 template <typename T>
 void param_final(const typename Storage<T>::acc* sums, int64_t blocks, int len, void* dw, void* db, bool f32,
                  cudaStream_t stream) {
-    norm_param_final_kernel<T><<<ceil_div(len, 32), kParamThreads, 0, stream>>>(sums, blocks, len, dw, db, f32);
+    // no more shares than partial sums
+    int threads = 32;
+    while (threads < kParamThreads && threads / 32 < blocks) threads *= 2;
+    norm_param_final_kernel<T><<<static_cast<unsigned>(ceil_div64(2ll * len, 32)), threads, 0, stream>>>(
+        sums, static_cast<int>(blocks), len, dw, db, f32);
     SB_CUDA(cudaGetLastError());
 }
 
@@ -220,6 +225,7 @@ void norm_forward(const char* name, const Norm& n, const void* x_, const void* w
             a.eps = static_cast<float>(eps);
             a.shape = n.shape;
             a.rule = rule;
+            a.stats_wide = fits(sizeof(float) * p.V, a.mean, a.rstd);
             a.tiles = p.tiles;
             SB_CUDA(norm_launch<T>(p, false, join, a, stream));
             return;
@@ -270,6 +276,7 @@ void norm_backward(const char* name, const Norm& n, const void* gy_, const void*
             a.part = dw || db ? reinterpret_cast<float*>(ws) : nullptr;
             a.shape = n.shape;
             a.rule = rule;
+            a.stats_wide = fits(sizeof(float) * p.V, a.mean, a.rstd);
             a.tiles = p.tiles;
             SB_CUDA(norm_launch<T>(p, true, join, a, stream));
             if (dw || db) param_final<T>(a.part, p.blocks, n.shape.len, dw, db, f32, stream);
