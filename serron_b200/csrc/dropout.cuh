@@ -18,7 +18,7 @@ __global__ void __launch_bounds__(256)
     using F = Floats<V>;
     const long long start = blockIdx.x * (256ll * U * V);
     const uint32_t high = static_cast<uint32_t>(start >> 34), low = static_cast<uint32_t>(start >> 2);
-    const float scale = static_cast<float>(rule.scale);
+    const float scale = rule.scale32;
     PhiloxKeys own;
     if (DEVICE_SEED) own.set(__ldg(rule.seed_device));
     const PhiloxKeys& keys = DEVICE_SEED ? own : rule.keys;
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256)
     const int left = static_cast<int>(min(span - at, 256ll * U * V));
     const bool kept =
         word_of(philox(unit >> 2, rule.sequence, rule.own_keys()), unit & 3) >= rule.threshold && !rule.all;
-    const float scale = static_cast<float>(rule.scale);
+    const float scale = rule.scale32;
     P in[U], res[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {

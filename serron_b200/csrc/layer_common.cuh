@@ -17,14 +17,14 @@ constexpr int kPhiloxRounds = 10;
 constexpr uint32_t kPhiloxMul0 = 0xD2511F53u, kPhiloxMul1 = 0xCD9E8D57u;
 constexpr uint32_t kPhiloxKey0 = 0x9E3779B9u, kPhiloxKey1 = 0xBB67AE85u;
 
-// The keys of all rounds.
-struct PhiloxKeys {
-    uint32_t k0[kPhiloxRounds], k1[kPhiloxRounds];
+// The keys of all rounds, both words of a round side by side.
+struct alignas(16) PhiloxKeys {
+    uint32_t k[2 * kPhiloxRounds];
 
     __host__ __device__ __forceinline__ void set(uint64_t seed) {
         for (int r = 0; r < kPhiloxRounds; ++r) {
-            k0[r] = static_cast<uint32_t>(seed) + r * kPhiloxKey0;
-            k1[r] = static_cast<uint32_t>(seed >> 32) + r * kPhiloxKey1;
+            k[2 * r] = static_cast<uint32_t>(seed) + r * kPhiloxKey0;
+            k[2 * r + 1] = static_cast<uint32_t>(seed >> 32) + r * kPhiloxKey1;
         }
     }
 };
@@ -38,9 +38,9 @@ __device__ __forceinline__ uint4 philox(uint32_t low, uint32_t high, uint64_t se
     for (int r = 0; r < kPhiloxRounds; ++r) {
         const uint64_t a = static_cast<uint64_t>(c0) * kPhiloxMul0;
         const uint64_t b = static_cast<uint64_t>(c2) * kPhiloxMul1;
-        c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ keys.k0[r];
+        c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ keys.k[2 * r];
         c1 = static_cast<uint32_t>(b);
-        c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ keys.k1[r];
+        c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ keys.k[2 * r + 1];
         c3 = static_cast<uint32_t>(a);
     }
     return make_uint4(c0, c1, c2, c3);
@@ -61,6 +61,7 @@ struct DropRule {
     uint32_t threshold = 0;  // round(p * 2^32)
     bool all = false;        // p rounds to one: every element is dropped
     double scale = 1.0;      // 1 / (1 - p)
+    float scale32 = 1.0f;
 
     // the keys wherever the seed is (in registers)
     __device__ __forceinline__ PhiloxKeys own_keys() const {

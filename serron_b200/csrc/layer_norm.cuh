@@ -252,30 +252,31 @@ __global__ void __launch_bounds__(kNormThreads)
     }
 }
 
-// Each block: 32 of the 2 * len columns (dw, then db), blockDim.x / 32 shares of the partial sums.
+// A block sums blockDim.x of the 2 * len columns (dw, then db), each in blockDim.y shares of the partial sums.
 constexpr int kParamThreads = 1024;
 template <typename T>
 __global__ void __launch_bounds__(kParamThreads)
     norm_param_final_kernel(const typename Storage<T>::acc* __restrict__ part, int blocks, int len,
                             void* __restrict__ dw, void* __restrict__ db, bool f32) {
-    __shared__ double shared[kParamThreads / 32][33];
-    const int lane = threadIdx.x & 31, share = threadIdx.x >> 5, shares = blockDim.x >> 5;
-    const long long width = 2ll * len, column = blockIdx.x * 32ll + lane;
+    __shared__ double shared[kParamThreads];
+    const int shares = blockDim.y, at = threadIdx.y * blockDim.x + threadIdx.x;
+    const long long width = 2ll * len, column = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
     double sum = 0.0;
     if (column < width) {
         const typename Storage<T>::acc* p = part + column;
 #pragma unroll 8
-        for (int k = share; k < blocks; k += shares) sum += p[k * width];
+        for (int k = threadIdx.y; k < blocks; k += shares) sum += p[k * width];
     }
-    shared[share][lane] = sum;
-    __syncthreads();
-    // a warp joins the shares of one column at a time
-    for (int i = share; i < 32; i += shares) {
-        const double total = warp_sum(lane < shares ? shared[lane][i] : 0.0);
-        const long long c = blockIdx.x * 32ll + i;
-        void* out = c < len ? dw : db;
-        if (lane == 0 && c < width && out != nullptr) store_param<T>(out, c < len ? c : c - len, f32, total);
+    if (shares > 1) {
+        shared[at] = sum;
+        for (int half = shares >> 1; half > 0; half >>= 1) {  // a power of two of shares
+            __syncthreads();
+            if (threadIdx.y < half) shared[at] = sum += shared[at + half * blockDim.x];
+        }
     }
+    void* out = column < len ? dw : db;
+    if (threadIdx.y == 0 && column < width && out != nullptr)
+        store_param<T>(out, column < len ? column : column - len, f32, sum);
 }
 
 }  // namespace serron

@@ -9,9 +9,8 @@
 //   columns  (inner  > 1): threadIdx.x counts vectors of V neighbouring rows (neighbours in memory), threadIdx.y the
 //            strides of the normalised dimension
 //
-// Forward: a part of a row (a thread's, a warp's or a block's) gives its sum S and the sum Q of squared distances from a
-// pivot near its mean; parts of n elements join as  mean = sum S / len  and  sum of squares about it =
-// sum (Q + n (pivot - mean)^2),  so a level far above the spread costs nothing.  Backward: two plain sums.
+// The forward pass adds up a row twice over its registers, for the mean and for the squares about that mean, so that a level far
+// above the spread costs nothing; the backward pass adds up two numbers once.
 //
 // These kernels would be bound by instructions, not by memory, if written one float at a time (31 instructions an element
 // of a row, 48 of a column, where 16-bit elements leave about 20 at the memory's rate): elements are unpacked
@@ -52,9 +51,10 @@ struct NormArgs {
 };
 
 // s / n where `inverse` is 1 / n: exact where the quotient is a float.
-__device__ __forceinline__ float quotient(float s, float n, float inverse) {
-    const float q = s * inverse;
-    return fmaf(fmaf(-n, q, s), inverse, q);
+template <typename E>
+__device__ __forceinline__ E quotient(E s, float n, float inverse) {
+    const E q = mul(s, splat<E>(inverse));
+    return fma(fma(splat<E>(-n), q, s), splat<E>(inverse), q);
 }
 
 // 1 / sqrt(v): the approximation and one Newton step (infinite v: zero, as 1 / sqrt gives).
@@ -64,20 +64,14 @@ __device__ __forceinline__ float root_inverse(float v) {
     return v < __int_as_float(0x7f800000) ? better : r;
 }
 
-// How many of the positions first, first + step, ... lie below len, for any first < step: one division for all.
-struct CountBelow {
-    int whole, rest;
-    __device__ __forceinline__ CountBelow(int step, int len) : whole(len / step), rest(len - len / step * step) {}
-    __device__ __forceinline__ int operator()(int first) const { return whole + (first < rest); }
-};
-
 // The generator's keys, in shared memory: a launch takes its seed from the host or from device memory.
 __device__ __forceinline__ void share_keys(const DropRule& rule, PhiloxKeys& shared) {
     const int r = threadIdx.y * blockDim.x + threadIdx.x;
     if (r < kPhiloxRounds) {
         const uint64_t seed = rule.seed_device ? __ldg(rule.seed_device) : 0;
-        shared.k0[r] = rule.seed_device ? static_cast<uint32_t>(seed) + r * kPhiloxKey0 : rule.keys.k0[r];
-        shared.k1[r] = rule.seed_device ? static_cast<uint32_t>(seed >> 32) + r * kPhiloxKey1 : rule.keys.k1[r];
+        shared.k[2 * r] = rule.seed_device ? static_cast<uint32_t>(seed) + r * kPhiloxKey0 : rule.keys.k[2 * r];
+        shared.k[2 * r + 1] =
+            rule.seed_device ? static_cast<uint32_t>(seed >> 32) + r * kPhiloxKey1 : rule.keys.k[2 * r + 1];
     }
     __syncthreads();
 }
@@ -93,33 +87,46 @@ __device__ __forceinline__ Floats<V> drop(const Floats<V>& v, long long e, const
     }
     uint32_t words[V];
     drop_words<V>(e, rule.sequence, keys, words);
-    return dropped<V>(v, words, rule.threshold, static_cast<float>(rule.scale));
+    return dropped<V>(v, words, rule.threshold, rule.scale32);
 }
 
-// h = residual + dropout(x), rounded to T and stored.
+// residual + dropout(x), rounded to T
 template <typename T, int V>
-__device__ __forceinline__ Floats<V> join_at(const Pack<T, V>& x, const Pack<T, V>& residual, long long e,
-                                             const DropRule& rule, const PhiloxKeys& keys, T* sum) {
+__device__ __forceinline__ Pack<T, V> joined(const Pack<T, V>& x, const Pack<T, V>& residual, long long e,
+                                             const DropRule& rule, const PhiloxKeys& keys) {
     Floats<V> v = drop<V>(x.floats(), e, rule, keys);
     const Floats<V> r = residual.floats();
 #pragma unroll
     for (int i = 0; i < Floats<V>::N; ++i) v.e[i] = add(v.e[i], r.e[i]);
-    const Pack<T, V> out = Pack<T, V>::of(v);
-    out.store(sum + e);
-    return out.floats();
+    return Pack<T, V>::of(v);
 }
 
-// What follows dx = v in memory order from e on: the sum with `add`, dx itself, and its masked copy.
+// V elements at p; of an incomplete vector only those from lo to hi.
+template <typename T, int V>
+__device__ __forceinline__ void store_part(T* p, const Pack<T, V>& v, bool whole, int lo, int hi) {
+    if (whole) {
+        v.store(p);
+    } else {
+        float f[V];
+        v.floats().to(f);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i >= lo && i < hi) p[i] = Storage<T>::store(f[i]);
+    }
+}
+
+// What follows dx = v from element e on: the sum with `extra`, dx itself, and its masked copy.
 template <typename T, int V, bool JOIN>
 __device__ __forceinline__ void store_dx(Floats<V> v, long long e, const NormArgs<T>& a, const Pack<T, V>& extra,
-                                         const PhiloxKeys& keys) {
+                                         const PhiloxKeys& keys, bool whole = true, int lo = 0, int hi = V) {
     if (JOIN && a.add != nullptr) {
         const Floats<V> f = extra.floats();
 #pragma unroll
         for (int i = 0; i < Floats<V>::N; ++i) v.e[i] = add(v.e[i], f.e[i]);
     }
-    if (a.dx != nullptr) Pack<T, V>::of(v).store(a.dx + e);
-    if (JOIN && a.dropped != nullptr) Pack<T, V>::of(drop<V>(v, e, a.rule, keys)).store(a.dropped + e);
+    if (a.dx != nullptr) store_part<T, V>(a.dx + e, Pack<T, V>::of(v), whole, lo, hi);
+    if (JOIN && a.dropped != nullptr)
+        store_part<T, V>(a.dropped + e, Pack<T, V>::of(drop<V>(v, e, a.rule, keys)), whole, lo, hi);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -149,6 +156,51 @@ __device__ __forceinline__ Floats<V> got(const float* plane, int lane) {
     return Pack<float, V>::load(plane + lane * V).floats();
 }
 
+// Sums M numbers for each of a lane's V rows over the groups of a block, then over the blocks of a cluster.  `shared`:
+// [2 phases][M][groups][lanes][V], then for the cluster [2 phases][M][lanes][V]; `phase` alternates from call to call, so that a
+// call's reads and the next but one's writes have a barrier between them.
+template <int V, int M>
+__device__ __forceinline__ void column_totals(Floats<V> (&v)[M], float* shared, int& phase) {
+    const int lanes = blockDim.x, groups = blockDim.y, lane = threadIdx.x, clusters = gridDim.y, plane = lanes * V;
+    if (groups > 1) {
+        float* mine = shared + phase * M * groups * plane;
+#pragma unroll
+        for (int m = 0; m < M; ++m) put<V>(mine + (m * groups + threadIdx.y) * plane, lane, v[m]);
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < M; ++m) v[m] = got<V>(mine + m * groups * plane, lane);
+        for (int g = 1; g < groups; ++g) {
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                const Floats<V> p = got<V>(mine + (m * groups + g) * plane, lane);
+#pragma unroll
+                for (int i = 0; i < Floats<V>::N; ++i) v[m].e[i] = add(v[m].e[i], p.e[i]);
+            }
+        }
+    }
+    if (clusters > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        float* mine = shared + (2 * groups + phase) * M * plane;
+        if (threadIdx.y == 0) {
+#pragma unroll
+            for (int m = 0; m < M; ++m) put<V>(mine + m * plane, lane, v[m]);
+        }
+        cluster.sync();
+#pragma unroll
+        for (int m = 0; m < M; ++m) v[m].fill(0.0f);
+        for (int c = 0; c < clusters; ++c) {
+            const float* theirs = cluster.map_shared_rank(mine, c);
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                const Floats<V> p = got<V>(theirs + m * plane, lane);
+#pragma unroll
+                for (int i = 0; i < Floats<V>::N; ++i) v[m].e[i] = add(v[m].e[i], p.e[i]);
+            }
+        }
+    }
+    phase ^= 1;
+}
+
 // FULL: every thread has all of its NV strides (len is their number times the groups').
 template <typename T, int V, int NV, bool JOIN, bool FULL>
 __global__ void __launch_bounds__(512, 1) norm_columns_kernel(const __grid_constant__ NormArgs<T> a) {
@@ -156,17 +208,14 @@ __global__ void __launch_bounds__(512, 1) norm_columns_kernel(const __grid_const
     using F = Floats<V>;
     using E = typename F::E;
     constexpr int N = F::N;
-    // [2 tiles][2][groups][lanes][V], then for the cluster [2 tiles][2][lanes][V]
     extern __shared__ __align__(16) float shared[];
     __shared__ PhiloxKeys keys;
-    const int lanes = blockDim.x, groups = blockDim.y, lane = threadIdx.x;
-    const int clusters = gridDim.y, all = groups * clusters;
-    const int group = blockIdx.y * groups + threadIdx.y;
-    const int len = a.shape.len, plane = lanes * V;
+    const int lanes = blockDim.x, lane = threadIdx.x;
+    const int clusters = gridDim.y, all = blockDim.y * clusters;
+    const int group = blockIdx.y * blockDim.y + threadIdx.y;
+    const int len = a.shape.len;
     const long long step = static_cast<long long>(all) * a.shape.inner;
-    const CountBelow below(all, len);
-    const int count = FULL ? NV : below(group);
-    const float part_inverse = 1.0f / static_cast<float>(max(count, 1)), len_inverse = 1.0f / static_cast<float>(len);
+    const float n = static_cast<float>(len), inverse = 1.0f / n;
     if (JOIN) share_keys(a.rule, keys);
 
     float w[NV], b[NV];
@@ -177,166 +226,85 @@ __global__ void __launch_bounds__(512, 1) norm_columns_kernel(const __grid_const
         b[k] = (FULL || c < len) && a.bias ? load_param<T>(a.bias, c, a.f32) : 0.0f;
     }
 
-    int parity = 0;
-    for (long long t = blockIdx.x; t < a.tiles; t += gridDim.x, parity ^= 1) {
+    int phase = 0;
+    for (long long t = blockIdx.x; t < a.tiles; t += gridDim.x) {
         const long long q = t * lanes + lane;
         long long offset;
         const bool live = column_place<V>(a.shape, q, offset);
         const long long first = offset + static_cast<long long>(group) * a.shape.inner;
-        F h[NV];
-        {
-            P in[NV], res[JOIN ? NV : 1];
-            if (live) {
+        P h[NV];
+        F sum[1], squares[1];
+        sum[0].fill(0.0f);
+        squares[0].fill(0.0f);
+        if (live) {
+            P res[JOIN ? NV : 1];
 #pragma unroll
-                for (int k = 0; k < NV; ++k) {
-                    if (FULL || group + k * all < len) {
-                        in[k] = P::load(a.x + first + k * step);
-                        if (JOIN) res[k] = P::load(a.residual + first + k * step);
-                    }
+            for (int k = 0; k < NV; ++k) {
+                if (FULL || group + k * all < len) {
+                    h[k] = P::load(a.x + first + k * step);
+                    if (JOIN) res[k] = P::load(a.residual + first + k * step);
                 }
             }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                if (live && (FULL || group + k * all < len)) {
-                    if (JOIN)
-                        h[k] = join_at<T, V>(in[k], res[k], first + k * step, a.rule, keys, a.sum);
-                    else
-                        h[k] = in[k].floats();
-                } else {
-                    h[k].fill(0.0f);
+                if (FULL || group + k * all < len) {
+                    if (JOIN) {
+                        h[k] = joined<T, V>(h[k], res[k], first + k * step, a.rule, keys);
+                        h[k].store(a.sum + first + k * step);
+                    }
+                    const F f = h[k].floats();
+#pragma unroll
+                    for (int i = 0; i < N; ++i) sum[0].e[i] = add(sum[0].e[i], f.e[i]);
                 }
             }
         }
-        // the thread's part of each row: sum, and squares about its mean
-        F sum, squares, mean;
-        sum.fill(0.0f);
-        squares.fill(0.0f);
+        column_totals<V, 1>(sum, shared, phase);
+        F mean;
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+        for (int i = 0; i < N; ++i) mean.e[i] = quotient(sum[0].e[i], n, inverse);
+        if (live) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum.e[i] = add(sum.e[i], h[k].e[i]);
-        if (all == 1) {
-            float s[V];
-            sum.to(s);
+            for (int k = 0; k < NV; ++k) {
+                if (FULL || group + k * all < len) {
+                    const F f = h[k].floats();
 #pragma unroll
-            for (int v = 0; v < V; ++v) s[v] = quotient(s[v], static_cast<float>(len), len_inverse);
-            mean.from(s);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) mean.e[i] = mul(sum.e[i], splat<E>(part_inverse));
-        }
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            if (FULL || group + k * all < len) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const E d = sub(h[k].e[i], mean.e[i]);
-                    squares.e[i] = fma(d, d, squares.e[i]);
-                }
-            }
-        }
-        if (groups > 1) {
-            float* sums = shared + parity * 2 * groups * plane;
-            float* sqs = sums + groups * plane;
-            put<V>(sums + threadIdx.y * plane, lane, sum);
-            put<V>(sqs + threadIdx.y * plane, lane, squares);
-            __syncthreads();
-            // the block's part: its groups are blockIdx.y * groups .. + groups - 1
-            sum.fill(0.0f);
-            int held = 0;
-            for (int g = 0; g < groups; ++g) {
-                const F s = got<V>(sums + g * plane, lane);
-                held += below(blockIdx.y * groups + g);
-#pragma unroll
-                for (int i = 0; i < N; ++i) sum.e[i] = add(sum.e[i], s.e[i]);
-            }
-            const float n = static_cast<float>(max(held, 1)), n_inverse = clusters == 1 ? len_inverse : 1.0f / n;
-            float m[V];
-            sum.to(m);
-#pragma unroll
-            for (int v = 0; v < V; ++v) m[v] = quotient(m[v], n, n_inverse);
-            mean.from(m);
-            squares.fill(0.0f);
-            const float more_inverse = 1.0f / static_cast<float>(below.whole + 1);
-            const float whole_inverse = 1.0f / static_cast<float>(max(below.whole, 1));
-            for (int g = 0; g < groups; ++g) {
-                const bool more = blockIdx.y * groups + g < below.rest;
-                const float gn = static_cast<float>(below.whole + more), inverse = more ? more_inverse : whole_inverse;
-                const F s = got<V>(sums + g * plane, lane), sq = got<V>(sqs + g * plane, lane);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const E d = sub(mul(s.e[i], splat<E>(inverse)), mean.e[i]);
-                    squares.e[i] = add(squares.e[i], fma(mul(d, splat<E>(gn)), d, sq.e[i]));
-                }
-            }
-        }
-        if (clusters > 1) {
-            cg::cluster_group cluster = cg::this_cluster();
-            float* mine = shared + (4 * groups + parity * 2) * plane;
-            if (threadIdx.y == 0) {
-                put<V>(mine, lane, sum);
-                put<V>(mine + plane, lane, squares);
-            }
-            cluster.sync();
-            sum.fill(0.0f);
-            for (int c = 0; c < clusters; ++c) {
-                const F s = got<V>(cluster.map_shared_rank(mine, c), lane);
-#pragma unroll
-                for (int i = 0; i < N; ++i) sum.e[i] = add(sum.e[i], s.e[i]);
-            }
-            float m[V];
-            sum.to(m);
-#pragma unroll
-            for (int v = 0; v < V; ++v) m[v] = quotient(m[v], static_cast<float>(len), len_inverse);
-            mean.from(m);
-            squares.fill(0.0f);
-            for (int c = 0; c < clusters; ++c) {
-                const float* theirs = cluster.map_shared_rank(mine, c);
-                const F s = got<V>(theirs, lane), sq = got<V>(theirs + plane, lane);
-                const float n = static_cast<float>(
-                    max(groups * below.whole + min(max(below.rest - c * groups, 0), groups), 1));
-                float ms[V];
-                s.to(ms);
-#pragma unroll
-                for (int v = 0; v < V; ++v) ms[v] = quotient(ms[v], n, 1.0f / n);
-                F d;
-                d.from(ms);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const E e = sub(d.e[i], mean.e[i]);
-                    squares.e[i] = add(squares.e[i], fma(mul(e, splat<E>(n)), e, sq.e[i]));
-                }
-            }
-        }
-        if (!live) continue;
-        F rstd;
-        {
-            float m[V], r[V];
-            mean.to(m);
-            squares.to(r);
-#pragma unroll
-            for (int v = 0; v < V; ++v) r[v] = root_inverse(fmaf(r[v], len_inverse, a.eps));
-            rstd.from(r);
-            if (a.mean != nullptr && group == 0) {
-                if (a.stats_wide) {
-                    put<V>(a.mean + q * V, 0, mean);
-                    put<V>(a.rstd + q * V, 0, rstd);
-                } else {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        a.mean[q * V + v] = m[v];
-                        a.rstd[q * V + v] = r[v];
+                    for (int i = 0; i < N; ++i) {
+                        const E d = sub(f.e[i], mean.e[i]);
+                        squares[0].e[i] = fma(d, d, squares[0].e[i]);
                     }
                 }
             }
         }
+        column_totals<V, 1>(squares, shared, phase);
+        if (!live) continue;
+        F rstd;
+        float r[V];
+        squares[0].to(r);
+#pragma unroll
+        for (int v = 0; v < V; ++v) r[v] = root_inverse(fmaf(r[v], inverse, a.eps));
+        rstd.from(r);
+        if (a.mean != nullptr && group == 0) {
+            if (a.stats_wide) {
+                put<V>(a.mean + q * V, 0, mean);
+                put<V>(a.rstd + q * V, 0, rstd);
+            } else {
+                float m[V];
+                mean.to(m);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    a.mean[q * V + v] = m[v];
+                    a.rstd[q * V + v] = r[v];
+                }
+            }
+        }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             if (FULL || group + k * all < len) {
+                const F f = h[k].floats();
                 F out;
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    out.e[i] = fma(mul(sub(h[k].e[i], mean.e[i]), rstd.e[i]), splat<E>(w[k]), splat<E>(b[k]));
+                    out.e[i] = fma(mul(sub(f.e[i], mean.e[i]), rstd.e[i]), splat<E>(w[k]), splat<E>(b[k]));
                 P::of(out).store(a.y + first + k * step);
             }
         }
@@ -352,13 +320,12 @@ __global__ void __launch_bounds__(512, 1) norm_columns_bwd_kernel(const __grid_c
     using F = Floats<V>;
     using E = typename F::E;
     constexpr int N = F::N;
-    // [2 tiles][2][groups][lanes][V], then for the cluster [2 tiles][2][lanes][V]; at the end two floats a channel and warp
-    extern __shared__ __align__(16) float shared[];
+    extern __shared__ __align__(16) float shared[];  // column_totals'; at the end two floats a channel and warp
     __shared__ PhiloxKeys keys;
     const int lanes = blockDim.x, groups = blockDim.y, lane = threadIdx.x;
     const int clusters = gridDim.y, all = groups * clusters;
     const int group = blockIdx.y * groups + threadIdx.y;
-    const int len = a.shape.len, plane = lanes * V;
+    const int len = a.shape.len;
     const long long step = static_cast<long long>(all) * a.shape.inner;
     const float inverse = 1.0f / static_cast<float>(len);
     const bool stores = a.dx != nullptr || (JOIN && a.dropped != nullptr);
@@ -373,16 +340,16 @@ __global__ void __launch_bounds__(512, 1) norm_columns_bwd_kernel(const __grid_c
         dw[k] = db[k] = splat<E>(0.0f);
     }
 
-    int parity = 0;
-    for (long long t = blockIdx.x; t < a.tiles; t += gridDim.x, parity ^= 1) {
+    int phase = 0;
+    for (long long t = blockIdx.x; t < a.tiles; t += gridDim.x) {
         const long long q = t * lanes + lane;
         long long offset;
         const bool live = column_place<V>(a.shape, q, offset);
         const long long first = offset + static_cast<long long>(group) * a.shape.inner;
         P gy[NV], x[NV], extra[JOIN ? NV : 1];
-        F mean, rstd, s1, s2;
-        s1.fill(0.0f);
-        s2.fill(0.0f);
+        F mean, rstd, s[2];
+        s[0].fill(0.0f);
+        s[1].fill(0.0f);
         if (live) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
@@ -418,54 +385,20 @@ __global__ void __launch_bounds__(512, 1) norm_columns_bwd_kernel(const __grid_c
                         const E gx = mul(g.e[i], mul(sub(h.e[i], mean.e[i]), rstd.e[i]));
                         dw[k] = add(dw[k], gx);
                         db[k] = add(db[k], g.e[i]);
-                        s1.e[i] = fma(g.e[i], splat<E>(w[k]), s1.e[i]);
-                        s2.e[i] = fma(gx, splat<E>(w[k]), s2.e[i]);
+                        s[0].e[i] = fma(g.e[i], splat<E>(w[k]), s[0].e[i]);
+                        s[1].e[i] = fma(gx, splat<E>(w[k]), s[1].e[i]);
                     }
                 }
             }
         }
-        if (groups > 1) {
-            float* sums = shared + parity * 2 * groups * plane;
-            float* sums2 = sums + groups * plane;
-            put<V>(sums + threadIdx.y * plane, lane, s1);
-            put<V>(sums2 + threadIdx.y * plane, lane, s2);
-            __syncthreads();
-            s1.fill(0.0f);
-            s2.fill(0.0f);
-            for (int g = 0; g < groups; ++g) {
-                const F p1 = got<V>(sums + g * plane, lane), p2 = got<V>(sums2 + g * plane, lane);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    s1.e[i] = add(s1.e[i], p1.e[i]);
-                    s2.e[i] = add(s2.e[i], p2.e[i]);
-                }
-            }
-        }
-        if (clusters > 1) {
-            cg::cluster_group cluster = cg::this_cluster();
-            float* mine = shared + (4 * groups + parity * 2) * plane;
-            if (threadIdx.y == 0) {
-                put<V>(mine, lane, s1);
-                put<V>(mine + plane, lane, s2);
-            }
-            cluster.sync();
-            s1.fill(0.0f);
-            s2.fill(0.0f);
-            for (int c = 0; c < clusters; ++c) {
-                const float* theirs = cluster.map_shared_rank(mine, c);
-                const F p1 = got<V>(theirs, lane), p2 = got<V>(theirs + plane, lane);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    s1.e[i] = add(s1.e[i], p1.e[i]);
-                    s2.e[i] = add(s2.e[i], p2.e[i]);
-                }
-            }
-        }
+        column_totals<V, 2>(s, shared, phase);
         if (live && stores) {
+            // dx = rstd (g w - mean(g w) - xhat mean(g w xhat)), with rstd multiplied into what is the same for a row
+            F scale, shift;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                s1.e[i] = mul(s1.e[i], splat<E>(-inverse));
-                s2.e[i] = mul(s2.e[i], splat<E>(-inverse));
+                shift.e[i] = mul(mul(s[0].e[i], splat<E>(-inverse)), rstd.e[i]);
+                scale.e[i] = mul(mul(s[1].e[i], splat<E>(-inverse)), mul(rstd.e[i], rstd.e[i]));
             }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
@@ -473,10 +406,9 @@ __global__ void __launch_bounds__(512, 1) norm_columns_bwd_kernel(const __grid_c
                     const F g = gy[k].floats(), h = x[k].floats();
                     F d;
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const E xhat = mul(sub(h.e[i], mean.e[i]), rstd.e[i]);
-                        d.e[i] = mul(rstd.e[i], fma(xhat, s2.e[i], fma(g.e[i], splat<E>(w[k]), s1.e[i])));
-                    }
+                    for (int i = 0; i < N; ++i)
+                        d.e[i] = fma(mul(g.e[i], splat<E>(w[k])), rstd.e[i],
+                                     fma(sub(h.e[i], mean.e[i]), scale.e[i], shift.e[i]));
                     store_dx<T, V, JOIN>(d, first + k * step, a, extra[JOIN ? k : 0], keys);
                 }
             }
@@ -520,247 +452,291 @@ __global__ void __launch_bounds__(512, 1) norm_columns_bwd_kernel(const __grid_c
 
 // ------------------------------------------------------------------------------------------------
 // rows
+//
+// blockDim.x threads a row: a power of two up to 32, or whole warps (then blockDim.y is 1).  Each group of threads takes
+// R rows at a time, whose loads are in flight together.
+//
+// Where V does not divide len (SHIFTED), vectors are laid over the memory and not over the row: the row's first
+// element is number `shift` of its first vector, and the first and the last vector hold elements of other rows, which
+// are put aside.  `shift` is the row's number times len, mod V, so a block takes rows that are V apart: they all have
+// the same, and a thread keeps the same elements of every row.
 // ------------------------------------------------------------------------------------------------
 
-// Sum over the `width` neighbouring lanes (a power of two up to 32) of a row.
-__device__ __forceinline__ float lanes_sum(float v, int width) {
-    for (int d = width >> 1; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    return v;
-}
-
-// blockDim.x threads a row: a power of two up to 32, or whole warps (then blockDim.y is 1).  Each group of threads
-// takes R rows at a time, whose loads are in flight together and which share the parameters' loads.
-template <typename T, int V, int NV, int R, bool JOIN>
-__global__ void __launch_bounds__(512, 1) norm_rows_kernel(const __grid_constant__ NormArgs<T> a) {
-    using P = Pack<T, V>;
-    using F = Floats<V>;
-    using E = typename F::E;
-    constexpr int N = F::N;
-    __shared__ float parts[16][R][2], counts[16], block[R][2];
-    __shared__ PhiloxKeys keys;
-    const int width = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int warps = width > 32 ? width >> 5 : 1;
-    const int clusters = gridDim.y, all = width * clusters;
-    const int len = a.shape.len, vectors = len / V;  // V divides len
-    const int first = blockIdx.y * width + threadIdx.x;
-    const float n = static_cast<float>(len), inverse = 1.0f / n;
-    const long long row = (blockIdx.x * static_cast<long long>(blockDim.y) + threadIdx.y) * R;
-    const long long base = row * len + static_cast<long long>(first) * V;
-    if (JOIN) share_keys(a.rule, keys);
-
-    F h[R][NV];
-    {
-        P in[R][NV], res[JOIN ? R : 1][NV];
+// Sums M numbers over the threads of a row: of a warp or a part of it, of a block, of a cluster.  Two phases, as above.
+template <int M>
+struct RowScratch {
+    float warps[2][16][M], block[2][M];
+};
+template <int M>
+__device__ __forceinline__ void row_totals(float (&v)[M], RowScratch<M>& scratch, int& phase) {
+    const int width = blockDim.x, clusters = gridDim.y;
+    if (width >= 32) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
+        for (int m = 0; m < M; ++m) v[m] = warp_sum(v[m]);
+    } else {
+        for (int d = width >> 1; d > 0; d >>= 1) {
 #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                if (row + r < a.shape.rows && first + k * all < vectors) {
-                    const long long e = base + static_cast<long long>(r) * len + k * all * V;
-                    in[r][k] = P::load(a.x + e);
-                    if (JOIN) res[r][k] = P::load(a.residual + e);
-                }
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-#pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                if (row + r < a.shape.rows && first + k * all < vectors) {
-                    const long long e = base + static_cast<long long>(r) * len + k * all * V;
-                    if (JOIN)
-                        h[r][k] = join_at<T, V>(in[r][k], res[r][k], e, a.rule, keys, a.sum);
-                    else
-                        h[r][k] = in[r][k].floats();
-                } else {
-                    h[r][k].fill(0.0f);
-                }
-            }
+            for (int m = 0; m < M; ++m) v[m] += __shfl_xor_sync(0xffffffffu, v[m], d);
         }
     }
-
-    float mean[R], squares[R];
+    if (width > 32) {
+        if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        E s = splat<E>(0.0f);
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int i = 0; i < N; ++i) s = add(s, h[r][k].e[i]);
-        mean[r] = total(s);
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) mean[r] = lanes_sum(mean[r], min(width, 32));
-    const bool whole = warps == 1 && clusters == 1;  // the warp has whole rows: their sums are what the mean is of
-    // the warp's elements of a row
-    float count = 0.0f, count_inverse = 0.0f;
-    if (!whole) {
-        int c = 0;
-#pragma unroll
-        for (int k = 0; k < NV; ++k) c += max(0, min(32, vectors - (first - lane) - k * all));
-        count = static_cast<float>(c * V);
-        count_inverse = 1.0f / fmaxf(count, 1.0f);
-    }
-    float sum[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        sum[r] = mean[r];
-        mean[r] = whole ? quotient(sum[r], n, inverse) : sum[r] * count_inverse;
-        const E m = splat<E>(mean[r]);
-        E q = splat<E>(0.0f);
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            if (first + k * all < vectors) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const E d = sub(h[r][k].e[i], m);
-                    q = fma(d, d, q);
-                }
-            }
-        }
-        squares[r] = total(q);
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) squares[r] = lanes_sum(squares[r], min(width, 32));
-    if (!whole) {
-        if (lane == 0) {
-            counts[warp] = count;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                parts[warp][r][0] = sum[r];
-                parts[warp][r][1] = squares[r];
-            }
+            for (int m = 0; m < M; ++m) scratch.warps[phase][threadIdx.x >> 5][m] = v[m];
         }
         __syncthreads();
-        float held = 0.0f;
-        for (int i = 0; i < warps; ++i) held += counts[i];
-        if (clusters == 1) held = n;
-        const float held_inverse = 1.0f / fmaxf(held, 1.0f);
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            sum[r] = squares[r] = 0.0f;
-            for (int i = 0; i < warps; ++i) sum[r] += parts[i][r][0];
-            mean[r] = quotient(sum[r], held, held_inverse);
-        }
-        for (int i = 0; i < warps; ++i) {
-            const float c = counts[i], c_inverse = 1.0f / fmaxf(c, 1.0f);
+        for (int m = 0; m < M; ++m) v[m] = scratch.warps[phase][0][m];
+        for (int i = 1; i < width >> 5; ++i) {
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const float d = parts[i][r][0] * c_inverse - mean[r];
-                squares[r] += fmaf(c * d, d, parts[i][r][1]);
-            }
+            for (int m = 0; m < M; ++m) v[m] += scratch.warps[phase][i][m];
         }
     }
     if (clusters > 1) {
         cg::cluster_group cluster = cg::this_cluster();
         if (threadIdx.x == 0) {
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                block[r][0] = sum[r];
-                block[r][1] = squares[r];
-            }
+            for (int m = 0; m < M; ++m) scratch.block[phase][m] = v[m];
         }
         cluster.sync();
 #pragma unroll
-        for (int r = 0; r < R; ++r) sum[r] = squares[r] = 0.0f;
+        for (int m = 0; m < M; ++m) v[m] = 0.0f;
         for (int c = 0; c < clusters; ++c) {
-            const float* theirs = cluster.map_shared_rank(&block[0][0], c);
+            const float* theirs = cluster.map_shared_rank(scratch.block[phase], c);
 #pragma unroll
-            for (int r = 0; r < R; ++r) sum[r] += theirs[2 * r];
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) mean[r] = quotient(sum[r], n, inverse);
-        for (int c = 0; c < clusters; ++c) {
-            const float* theirs = cluster.map_shared_rank(&block[0][0], c);
-            int held = 0;  // what block c has of a row
-#pragma unroll
-            for (int k = 0; k < NV; ++k) held += max(0, min(width, vectors - c * width - k * all));
-            const float cn = fmaxf(static_cast<float>(held) * V, 1.0f), c_inverse = 1.0f / cn;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const float d = quotient(theirs[2 * r], cn, c_inverse) - mean[r];
-                squares[r] += fmaf(cn * d, d, theirs[2 * r + 1]);
-            }
-        }
-        cluster.sync();  // no block leaves while another reads it
-    }
-    float rstd[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        rstd[r] = root_inverse(fmaf(squares[r], inverse, a.eps));
-        if (a.mean != nullptr && first == 0 && row + r < a.shape.rows) {
-            a.mean[row + r] = mean[r];
-            a.rstd[row + r] = rstd[r];
+            for (int m = 0; m < M; ++m) v[m] += theirs[m];
         }
     }
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int j = first + k * all;
-        if (j < vectors) {
-            F w, b;
-            w.fill(1.0f);
-            b.fill(0.0f);
-            if (a.weight) w = load_params<T, V>(a.weight, j * V, a.f32);
-            if (a.bias) b = load_params<T, V>(a.bias, j * V, a.f32);
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                if (row + r < a.shape.rows) {
-                    F out;
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        out.e[i] = fma(mul(sub(h[r][k].e[i], splat<E>(mean[r])), splat<E>(rstd[r])), w.e[i], b.e[i]);
-                    P::of(out).store(a.y + base + static_cast<long long>(r) * len + k * all * V);
-                }
-            }
-        }
-    }
+    phase ^= 1;
 }
 
-// The groups of a block walk over tiles of blockDim.y * R rows; a thread adds up its elements' parameter gradients on
-// the way.  `part` gets [gridDim.x][2][len] sums, one pair per block (cluster).
-template <typename T, int V, int NV, int R, bool JOIN>
-__global__ void __launch_bounds__(512, 1) norm_rows_bwd_kernel(const __grid_constant__ NormArgs<T> a) {
+// Where a thread of a row kernel stands: its vectors are first, first + all, ...
+template <int V, bool SHIFTED>
+struct RowPlace {
+    int shift, vectors, first, all, len;
+
+    __device__ __forceinline__ explicit RowPlace(const NormShape& s) {
+        len = s.len;
+        shift = SHIFTED ? static_cast<int>(static_cast<long long>(blockIdx.x % V) * len % V) : 0;
+        vectors = SHIFTED ? (len + shift + V - 1) / V : len / V;
+        all = blockDim.x * gridDim.y;
+        first = blockIdx.y * blockDim.x + threadIdx.x;
+    }
+    // the row of tile t that is the r-th of this thread's group
+    __device__ __forceinline__ long long row(long long t, int R, int r) const {
+        if (!SHIFTED) return (t * blockDim.y + threadIdx.y) * R + r;
+        return t % V + ((t / V * blockDim.y + threadIdx.y) * R + r) * V;
+    }
+    // the first element of its vector j in memory
+    __device__ __forceinline__ long long at(long long row, int j) const {
+        return row * len + (static_cast<long long>(j) * V - shift);
+    }
+    __device__ __forceinline__ int lo(int j) const { return SHIFTED && j == 0 ? shift : 0; }
+    __device__ __forceinline__ int hi(int j) const {
+        return SHIFTED && j == vectors - 1 ? len + shift - j * V : V;
+    }
+    __device__ __forceinline__ bool whole(int j) const {
+        return !SHIFTED || ((j > 0 || shift == 0) && len + shift - j * V >= V);
+    }
+    // the parameters of vector j's elements; `fill` beside the row
+    template <typename T>
+    __device__ __forceinline__ Floats<V> params(const void* p, int j, bool f32, float fill) const {
+        Floats<V> out;
+        if (p == nullptr) {
+            out.fill(fill);
+        } else if (!SHIFTED) {
+            out = load_params<T, V>(p, j * V, f32);
+        } else {
+            float f[V];
+            const int first_element = j * V - shift;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                f[i] = first_element + i >= 0 && first_element + i < len ? load_param<T>(p, first_element + i, f32) : fill;
+            out.from(f);
+        }
+        return out;
+    }
+};
+
+// The V elements from e on; those that lie before lo or from hi on read as zero where that is asked for (`whole` false).
+template <typename T, int V, bool SHIFTED>
+__device__ __forceinline__ Pack<T, V> load_part(const T* p, long long e, bool whole, int lo, int hi) {
+    if (!SHIFTED || whole) return Pack<T, V>::load(p + e);
+    float f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = i >= lo && i < hi ? Storage<T>::load(p[e + i]) : 0.0f;
+    Floats<V> v;
+    v.from(f);
+    return Pack<T, V>::of(v);
+}
+
+template <typename T, int V, int NV, int R, bool JOIN, bool SHIFTED>
+__global__ void __launch_bounds__(512, 1) norm_rows_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
     using F = Floats<V>;
     using E = typename F::E;
     constexpr int N = F::N;
-    __shared__ float parts[2][16][R][2], block[2][R][2];
-    extern __shared__ __align__(16) float sums[];  // [NV][threads][V] where a block has several groups
+    constexpr bool kKeepParams = SHIFTED && NV <= 2;  // unaligned parameters are read once
+    __shared__ RowScratch<R> scratch;
     __shared__ PhiloxKeys keys;
-    const int width = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int warps = width > 32 ? width >> 5 : 1;
-    const int clusters = gridDim.y, all = width * clusters;
-    const int len = a.shape.len, vectors = len / V;
-    const int first = blockIdx.y * width + threadIdx.x;
-    const float inverse = 1.0f / static_cast<float>(len);
+    const RowPlace<V, SHIFTED> place(a.shape);
+    const float n = static_cast<float>(place.len), inverse = 1.0f / n;
+    if (JOIN) share_keys(a.rule, keys);
+    F w[NV], b[NV];
+    if (kKeepParams) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            w[k] = place.template params<T>(a.weight, place.first + k * place.all, a.f32, 1.0f);
+            b[k] = place.template params<T>(a.bias, place.first + k * place.all, a.f32, 0.0f);
+        }
+    }
+
+    int phase = 0;
+    for (long long t = blockIdx.x; t < a.tiles; t += gridDim.x) {
+        P h[R][NV];
+        float sum[R], squares[R], mean[R], rstd[R];
+        {
+            P res[JOIN ? R : 1][NV];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const long long row = place.row(t, R, r);
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    const int j = place.first + k * place.all;
+                    if (row < a.shape.rows && j < place.vectors) {
+                        const long long e = place.at(row, j);
+                        const bool whole = place.whole(j);
+                        h[r][k] = load_part<T, V, SHIFTED>(a.x, e, whole, place.lo(j), place.hi(j));
+                        if (JOIN)
+                            res[r][k] = load_part<T, V, SHIFTED>(a.residual, e, whole, place.lo(j), place.hi(j));
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const long long row = place.row(t, R, r);
+                E s = splat<E>(0.0f);
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    const int j = place.first + k * place.all;
+                    if (row < a.shape.rows && j < place.vectors) {
+                        if (JOIN) {  // beside the row: dropout and sum of zeros
+                            const long long e = place.at(row, j);
+                            h[r][k] = joined<T, V>(h[r][k], res[r][k], e, a.rule, keys);
+                            store_part<T, V>(a.sum + e, h[r][k], place.whole(j), place.lo(j), place.hi(j));
+                        }
+                        const F f = h[r][k].floats();
+#pragma unroll
+                        for (int i = 0; i < N; ++i) s = add(s, f.e[i]);
+                    }
+                }
+                sum[r] = total(s);
+            }
+        }
+        row_totals<R>(sum, scratch, phase);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            mean[r] = quotient(sum[r], n, inverse);
+            E s = splat<E>(0.0f);
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int j = place.first + k * place.all;
+                if (place.row(t, R, r) < a.shape.rows && j < place.vectors) {
+                    F f = h[r][k].floats();
+#pragma unroll
+                    for (int i = 0; i < N; ++i) f.e[i] = sub(f.e[i], splat<E>(mean[r]));
+                    if (SHIFTED && !place.whole(j)) {
+                        float d[V];
+                        f.to(d);
+                        const int lo = place.lo(j), hi = place.hi(j);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) d[i] = i >= lo && i < hi ? d[i] : 0.0f;
+                        f.from(d);
+                    }
+#pragma unroll
+                    for (int i = 0; i < N; ++i) s = fma(f.e[i], f.e[i], s);
+                }
+            }
+            squares[r] = total(s);
+        }
+        row_totals<R>(squares, scratch, phase);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            rstd[r] = root_inverse(fmaf(squares[r], inverse, a.eps));
+            const long long row = place.row(t, R, r);
+            if (a.mean != nullptr && place.first == 0 && row < a.shape.rows) {
+                a.mean[row] = mean[r];
+                a.rstd[row] = rstd[r];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int j = place.first + k * place.all;
+            if (j < place.vectors) {
+                const F wk = kKeepParams ? w[k] : place.template params<T>(a.weight, j, a.f32, 1.0f);
+                const F bk = kKeepParams ? b[k] : place.template params<T>(a.bias, j, a.f32, 0.0f);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const long long row = place.row(t, R, r);
+                    if (row < a.shape.rows) {
+                        const F f = h[r][k].floats();
+                        F out;
+#pragma unroll
+                        for (int i = 0; i < N; ++i)
+                            out.e[i] = fma(mul(sub(f.e[i], splat<E>(mean[r])), splat<E>(rstd[r])), wk.e[i], bk.e[i]);
+                        store_part<T, V>(a.y + place.at(row, j), P::of(out), place.whole(j), place.lo(j), place.hi(j));
+                    }
+                }
+            }
+        }
+    }
+    if (gridDim.y > 1) cg::this_cluster().sync();  // no block leaves while another reads it
+}
+
+// `part` gets [gridDim.x][2][len] sums of the parameters' gradients, one pair per block (cluster).
+template <typename T, int V, int NV, int R, bool JOIN, bool SHIFTED>
+__global__ void __launch_bounds__(NV * V >= 32 ? 256 : 512, 1) norm_rows_bwd_kernel(const __grid_constant__ NormArgs<T> a) {
+    using P = Pack<T, V>;
+    using F = Floats<V>;
+    using E = typename F::E;
+    constexpr int N = F::N;
+    constexpr bool kKeepParams = SHIFTED && NV <= 2;
+    __shared__ RowScratch<2 * R> scratch;
+    extern __shared__ __align__(16) float sums[];  // [NV][V][threads] where a block has several groups
+    __shared__ PhiloxKeys keys;
+    const RowPlace<V, SHIFTED> place(a.shape);
+    const float inverse = 1.0f / static_cast<float>(place.len);
     const bool stores = a.dx != nullptr || (JOIN && a.dropped != nullptr);
     if (JOIN) share_keys(a.rule, keys);
 
-    F dw[NV], db[NV];
+    F dw[NV], db[NV], w[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         dw[k].fill(0.0f);
         db[k].fill(0.0f);
+        if (kKeepParams) w[k] = place.template params<T>(a.weight, place.first + k * place.all, a.f32, 1.0f);
     }
 
-    int parity = 0;
-    for (long long t = blockIdx.x; t < a.tiles; t += gridDim.x, parity ^= 1) {
-        const long long row = (t * blockDim.y + threadIdx.y) * R;
-        const long long base = row * len + static_cast<long long>(first) * V;
+    int phase = 0;
+    for (long long t = blockIdx.x; t < a.tiles; t += gridDim.x) {
         P gy[R][NV], x[R][NV], extra[JOIN ? R : 1][NV];
-        float mean[R], rstd[R], s1[R], s2[R];
+        float mean[R], rstd[R], s[2 * R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const bool live = row + r < a.shape.rows;
-            mean[r] = live ? a.mean[row + r] : 0.0f;
-            rstd[r] = live ? a.rstd[row + r] : 0.0f;
+            const long long row = place.row(t, R, r);
+            const bool live = row < a.shape.rows;
+            mean[r] = live ? a.mean[row] : 0.0f;
+            rstd[r] = live ? a.rstd[row] : 0.0f;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                if (live && first + k * all < vectors) {
-                    const long long e = base + static_cast<long long>(r) * len + k * all * V;
-                    gy[r][k] = P::load(a.gy + e);
-                    x[r][k] = P::load(a.x + e);
-                    if (JOIN && a.add != nullptr) extra[r][k] = P::load(a.add + e);
+                const int j = place.first + k * place.all;
+                if (live && j < place.vectors) {
+                    const long long e = place.at(row, j);
+                    const bool whole = place.whole(j);
+                    const int lo = place.lo(j), hi = place.hi(j);
+                    gy[r][k] = load_part<T, V, SHIFTED>(a.gy, e, whole, lo, hi);
+                    x[r][k] = load_part<T, V, SHIFTED>(a.x, e, whole, lo, hi);
+                    if (JOIN && a.add != nullptr) extra[r][k] = load_part<T, V, SHIFTED>(a.add, e, whole, lo, hi);
                 }
             }
         }
@@ -769,23 +745,20 @@ __global__ void __launch_bounds__(512, 1) norm_rows_bwd_kernel(const __grid_cons
         for (int r = 0; r < R; ++r) p1[r] = p2[r] = splat<E>(0.0f);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int j = first + k * all;
-            if (j < vectors) {
-                F w;
-                w.fill(1.0f);
-                if (a.weight) w = load_params<T, V>(a.weight, j * V, a.f32);
+            const int j = place.first + k * place.all;
+            if (j < place.vectors) {
+                const F wk = kKeepParams ? w[k] : place.template params<T>(a.weight, j, a.f32, 1.0f);
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    if (row + r < a.shape.rows) {
+                    if (place.row(t, R, r) < a.shape.rows) {
                         const F g = gy[r][k].floats(), h = x[r][k].floats();
 #pragma unroll
-                        for (int i = 0; i < N; ++i) {
-                            const E gx =
-                                mul(g.e[i], mul(sub(h.e[i], splat<E>(mean[r])), splat<E>(rstd[r])));
+                        for (int i = 0; i < N; ++i) {  // beside the row g is zero
+                            const E gx = mul(g.e[i], mul(sub(h.e[i], splat<E>(mean[r])), splat<E>(rstd[r])));
                             dw[k].e[i] = add(dw[k].e[i], gx);
                             db[k].e[i] = add(db[k].e[i], g.e[i]);
-                            p1[r] = fma(g.e[i], w.e[i], p1[r]);
-                            p2[r] = fma(gx, w.e[i], p2[r]);
+                            p1[r] = fma(g.e[i], wk.e[i], p1[r]);
+                            p2[r] = fma(gx, wk.e[i], p2[r]);
                         }
                     }
                 }
@@ -793,91 +766,54 @@ __global__ void __launch_bounds__(512, 1) norm_rows_bwd_kernel(const __grid_cons
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            s1[r] = lanes_sum(total(p1[r]), min(width, 32));
-            s2[r] = lanes_sum(total(p2[r]), min(width, 32));
+            s[2 * r] = total(p1[r]);
+            s[2 * r + 1] = total(p2[r]);
         }
-        if (warps > 1) {
-            if (lane == 0) {
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    parts[parity][warp][r][0] = s1[r];
-                    parts[parity][warp][r][1] = s2[r];
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int r = 0; r < R; ++r) s1[r] = s2[r] = 0.0f;
-            for (int i = 0; i < warps; ++i) {
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    s1[r] += parts[parity][i][r][0];
-                    s2[r] += parts[parity][i][r][1];
-                }
-            }
-        }
-        if (clusters > 1) {
-            cg::cluster_group cluster = cg::this_cluster();
-            if (threadIdx.x == 0) {
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    block[parity][r][0] = s1[r];
-                    block[parity][r][1] = s2[r];
-                }
-            }
-            cluster.sync();
-#pragma unroll
-            for (int r = 0; r < R; ++r) s1[r] = s2[r] = 0.0f;
-            for (int c = 0; c < clusters; ++c) {
-                const float* theirs = cluster.map_shared_rank(&block[parity][0][0], c);
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    s1[r] += theirs[2 * r];
-                    s2[r] += theirs[2 * r + 1];
-                }
-            }
-        }
+        row_totals<2 * R>(s, scratch, phase);
         if (stores) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const int j = first + k * all;
-                if (j < vectors) {
-                    F w;
-                    w.fill(1.0f);
-                    if (a.weight) w = load_params<T, V>(a.weight, j * V, a.f32);
+                const int j = place.first + k * place.all;
+                if (j < place.vectors) {
+                    const F wk = kKeepParams ? w[k] : place.template params<T>(a.weight, j, a.f32, 1.0f);
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        if (row + r < a.shape.rows) {
-                            const E m1 = splat<E>(-s1[r] * inverse), m2 = splat<E>(-s2[r] * inverse);
+                        const long long row = place.row(t, R, r);
+                        if (row < a.shape.rows) {
+                            const E shift = splat<E>(-s[2 * r] * inverse * rstd[r]);
+                            const E scale = splat<E>(-s[2 * r + 1] * inverse * (rstd[r] * rstd[r]));
                             const F g = gy[r][k].floats(), h = x[r][k].floats();
                             F d;
 #pragma unroll
-                            for (int i = 0; i < N; ++i) {
-                                const E xhat = mul(sub(h.e[i], splat<E>(mean[r])), splat<E>(rstd[r]));
-                                d.e[i] = mul(splat<E>(rstd[r]), fma(xhat, m2, fma(g.e[i], w.e[i], m1)));
-                            }
-                            store_dx<T, V, JOIN>(d, base + static_cast<long long>(r) * len + k * all * V, a,
-                                                 extra[JOIN ? r : 0][k], keys);
+                            for (int i = 0; i < N; ++i)
+                                d.e[i] = fma(mul(g.e[i], wk.e[i]), splat<E>(rstd[r]),
+                                             fma(sub(h.e[i], splat<E>(mean[r])), scale, shift));
+                            store_dx<T, V, JOIN>(d, place.at(row, j), a, extra[JOIN ? r : 0][k], keys, place.whole(j),
+                                                 place.lo(j), place.hi(j));
                         }
                     }
                 }
             }
         }
     }
-    if (clusters > 1) cg::this_cluster().sync();  // no block leaves while another reads it
+    if (gridDim.y > 1) cg::this_cluster().sync();  // no block leaves while another reads it
     if (a.part == nullptr) return;
-    const int groups = blockDim.y, threads = width * groups, tid = threadIdx.y * width + threadIdx.x;
+    const int len = place.len, width = blockDim.x, groups = blockDim.y;
+    const int threads = width * groups, tid = threadIdx.y * width + threadIdx.x;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         float* out = a.part + (blockIdx.x * 2ll + which) * len;
         if (groups == 1) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const int j = first + k * all;
-                if (j < vectors) {
+                const int j = place.first + k * place.all;
+                if (j < place.vectors) {
+                    const int lo = place.lo(j), hi = place.hi(j);
                     float v[V];
                     (which ? db : dw)[k].to(v);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) out[static_cast<long long>(j) * V + i] = v[i];
+                    for (int i = 0; i < V; ++i)
+                        if (!SHIFTED || (i >= lo && i < hi)) out[static_cast<long long>(j) * V + i - place.shift] = v[i];
                 }
             }
         } else {  // several groups, no cluster
@@ -891,11 +827,11 @@ __global__ void __launch_bounds__(512, 1) norm_rows_bwd_kernel(const __grid_cons
             }
             __syncthreads();
             for (int l = tid; l < len; l += threads) {
-                const int j = l / V, k = j / width;
-                const float* from = sums + (k * V + l % V) * threads + (j - k * width);
-                float s = 0.0f;
-                for (int g = 0; g < groups; ++g) s += from[g * width];
-                out[l] = s;
+                const int p = l + place.shift, j = p / V, k = j / width;
+                const float* from = sums + (k * V + p % V) * threads + (j - k * width);
+                float sum = 0.0f;
+                for (int g = 0; g < groups; ++g) sum += from[g * width];
+                out[l] = sum;
             }
         }
     }

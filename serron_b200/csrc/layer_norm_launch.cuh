@@ -29,30 +29,29 @@ cudaError_t launch_norm(void (*kernel)(NormArgs<T>), const NormPlan& p, size_t s
     return cudaLaunchKernelEx(&config, kernel, args);
 }
 
-template <typename T, int V, int NV, int R>
+template <typename T, int V, int NV, int R, bool SHIFTED>
 cudaError_t launch_rows(const NormPlan& p, bool backward, bool join, const NormArgs<T>& args, cudaStream_t stream) {
     if (!backward)
-        return launch_norm<T>(join ? norm_rows_kernel<T, V, NV, R, true> : norm_rows_kernel<T, V, NV, R, false>, p, 0,
-                              args, stream);
-    if constexpr (NV * V <= 16) {
-        const size_t floats = p.ty > 1 ? size_t(NV) * V * p.tx * p.ty : 0;
-        return launch_norm<T>(join ? norm_rows_bwd_kernel<T, V, NV, R, true> : norm_rows_bwd_kernel<T, V, NV, R, false>,
-                              p, sizeof(float) * floats, args, stream);
-    }
-    return cudaErrorInvalidConfiguration;
+        return launch_norm<T>(
+            join ? norm_rows_kernel<T, V, NV, R, true, SHIFTED> : norm_rows_kernel<T, V, NV, R, false, SHIFTED>, p, 0,
+            args, stream);
+    const size_t floats = p.ty > 1 ? size_t(NV) * V * p.tx * p.ty : 0;
+    return launch_norm<T>(
+        join ? norm_rows_bwd_kernel<T, V, NV, R, true, SHIFTED> : norm_rows_bwd_kernel<T, V, NV, R, false, SHIFTED>, p,
+        sizeof(float) * floats, args, stream);
 }
 
 template <typename T, int V, int NV, bool FULL>
 cudaError_t launch_columns(const NormPlan& p, bool backward, bool join, const NormArgs<T>& args, cudaStream_t stream) {
-    // two tiles' partial results: two per row and group, and two per row for the cluster
-    const size_t floats = (p.ty > 1 || p.clusters > 1) ? (4 * size_t(p.ty) + 4) * p.tx * V : 0;
+    // column_totals' scratch for one number a row, for two in a backward pass
+    const size_t floats = (p.ty > 1 || p.clusters > 1) ? (2 * size_t(p.ty) + 2) * p.tx * V : 0;
     if (!backward)
         return launch_norm<T>(
             join ? norm_columns_kernel<T, V, NV, true, FULL> : norm_columns_kernel<T, V, NV, false, FULL>, p,
             sizeof(float) * floats, args, stream);
     if constexpr (NV * V * sizeof(T) <= 64) {
         // at the end two sums per channel and warp
-        const size_t most = std::max(floats, size_t(NV) * p.ty * (p.tx / 32) * 2);
+        const size_t most = std::max(2 * floats, size_t(NV) * p.ty * (p.tx / 32) * 2);
         return launch_norm<T>(
             join ? norm_columns_bwd_kernel<T, V, NV, true, FULL> : norm_columns_bwd_kernel<T, V, NV, false, FULL>, p,
             sizeof(float) * most, args, stream);
@@ -60,33 +59,38 @@ cudaError_t launch_columns(const NormPlan& p, bool backward, bool join, const No
     return cudaErrorInvalidConfiguration;
 }
 
-// The kernel of plan `p`; the cases are those of norm_plan.
+// The kernel of plan `p`; the cases are those of plan_rows and plan_columns.
 template <typename T>
 cudaError_t norm_launch(const NormPlan& p, bool backward, bool join, const NormArgs<T>& args, cudaStream_t stream) {
     constexpr int W = 16 / sizeof(T);
-#define SERRON_ROWS_CASE(v, nv, r) \
-    if (p.V == v && p.NV == nv && p.R == r) return launch_rows<T, v, nv, r>(p, backward, join, args, stream);
+#define SERRON_ROWS_CASE(v, nv, r, off) \
+    if (p.V == v && p.NV == nv && p.R == r && p.shifted == off) \
+        return launch_rows<T, v, nv, r, off>(p, backward, join, args, stream);
 #define SERRON_COLUMNS_CASE(v, nv, whole) \
     if (p.V == v && p.NV == nv && p.full == whole) return launch_columns<T, v, nv, whole>(p, backward, join, args, stream);
     if (p.rows) {
-        SERRON_ROWS_CASE(W, 1, 4)
-        SERRON_ROWS_CASE(W, 1, 1)
-        SERRON_ROWS_CASE(W, 2, 2)
-        SERRON_ROWS_CASE(W, 2, 1)
-        SERRON_ROWS_CASE(W, 4, 1)
-        if constexpr (W == 8) {
-            SERRON_ROWS_CASE(2, 2, 4)
-            SERRON_ROWS_CASE(2, 2, 1)
-            SERRON_ROWS_CASE(2, 8, 1)
-        }
-        SERRON_ROWS_CASE(1, 4, 4)
-        SERRON_ROWS_CASE(1, 4, 1)
-        SERRON_ROWS_CASE(1, 16, 1)
+        SERRON_ROWS_CASE(W, 1, 4, false)
+        SERRON_ROWS_CASE(W, 1, 1, false)
+        SERRON_ROWS_CASE(W, 2, 2, false)
+        SERRON_ROWS_CASE(W, 2, 1, false)
+        SERRON_ROWS_CASE(W, 4, 1, false)
+        SERRON_ROWS_CASE(W, 1, 4, true)
+        SERRON_ROWS_CASE(W, 1, 1, true)
+        SERRON_ROWS_CASE(W, 2, 2, true)
+        SERRON_ROWS_CASE(W, 2, 1, true)
+        SERRON_ROWS_CASE(W, 4, 1, true)
+        SERRON_ROWS_CASE(1, 4, 4, false)
+        SERRON_ROWS_CASE(1, 4, 1, false)
+        SERRON_ROWS_CASE(1, 16, 1, false)
     } else {
         SERRON_COLUMNS_CASE(4, 4, true)
         SERRON_COLUMNS_CASE(4, 4, false)
         SERRON_COLUMNS_CASE(4, 8, true)
         SERRON_COLUMNS_CASE(4, 8, false)
+        if constexpr (sizeof(T) == 2) {
+            SERRON_COLUMNS_CASE(4, 16, true)
+            SERRON_COLUMNS_CASE(4, 16, false)
+        }
         SERRON_COLUMNS_CASE(1, 8, false)
         SERRON_COLUMNS_CASE(1, 16, false)
     }

@@ -52,6 +52,7 @@ DropRule drop_rule(const char* name, double p, uint64_t seed, const void* seed_d
     rule.all = threshold >= 4294967296.0;
     rule.threshold = rule.all ? 0xffffffffu : static_cast<uint32_t>(threshold);
     rule.scale = rule.all ? 0.0 : 1.0 / (1.0 - p);
+    rule.scale32 = static_cast<float>(rule.scale);
     return rule;
 }
 
@@ -193,11 +194,12 @@ bool params_fit(int V, bool f32, P... pointers) {
 template <typename T>
 void param_final(const typename Storage<T>::acc* sums, int64_t blocks, int len, void* dw, void* db, bool f32,
                  cudaStream_t stream) {
-    // no more shares than partial sums
-    int threads = 32;
-    while (threads < kParamThreads && threads / 32 < blocks) threads *= 2;
-    norm_param_final_kernel<T><<<static_cast<unsigned>(ceil_div64(2ll * len, 32)), threads, 0, stream>>>(
-        sums, static_cast<int>(blocks), len, dw, db, f32);
+    // eight partial sums or more to a share, at most 32 shares; at least a warp's width of columns
+    int shares = 1;
+    while (shares < 32 && blocks >= 16 * shares) shares *= 2;
+    const int columns = std::max(32, 128 / shares);
+    norm_param_final_kernel<T><<<static_cast<unsigned>(ceil_div64(2ll * len, columns)), dim3(columns, shares), 0,
+                                 stream>>>(sums, static_cast<int>(blocks), len, dw, db, f32);
     SB_CUDA(cudaGetLastError());
 }
 
