@@ -26,6 +26,7 @@ namespace serron {
 
 namespace cg = cooperative_groups;
 
+
 template <typename T>
 struct NormArgs {
     const T* x = nullptr;         // the input; the join's sum in the backward pass
@@ -203,7 +204,7 @@ __device__ __forceinline__ void column_totals(Floats<V> (&v)[M], float* shared, 
 
 // FULL: every thread has all of its NV strides (len is their number times the groups').
 template <typename T, int V, int NV, bool JOIN, bool FULL>
-__global__ void __launch_bounds__(512, 1) norm_columns_kernel(const __grid_constant__ NormArgs<T> a) {
+__global__ void __maxnreg__(JOIN ? 128 : 96) norm_columns_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
     using F = Floats<V>;
     using E = typename F::E;
@@ -214,7 +215,8 @@ __global__ void __launch_bounds__(512, 1) norm_columns_kernel(const __grid_const
     const int clusters = gridDim.y, all = blockDim.y * clusters;
     const int group = blockIdx.y * blockDim.y + threadIdx.y;
     const int len = a.shape.len;
-    const long long step = static_cast<long long>(all) * a.shape.inner;
+    const unsigned step = static_cast<unsigned>(all) * a.shape.inner;  // a sample's elements are counted in 31 bits here
+    const int count = (len - group + all - 1) / all;                    // of this thread's strides
     const float n = static_cast<float>(len), inverse = 1.0f / n;
     if (JOIN) share_keys(a.rule, keys);
 
@@ -222,8 +224,8 @@ __global__ void __launch_bounds__(512, 1) norm_columns_kernel(const __grid_const
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int c = group + k * all;
-        w[k] = (FULL || c < len) && a.weight ? load_param<T>(a.weight, c, a.f32) : 1.0f;
-        b[k] = (FULL || c < len) && a.bias ? load_param<T>(a.bias, c, a.f32) : 0.0f;
+        w[k] = (FULL || k < count) && a.weight ? load_param<T>(a.weight, c, a.f32) : 1.0f;
+        b[k] = (FULL || k < count) && a.bias ? load_param<T>(a.bias, c, a.f32) : 0.0f;
     }
 
     int phase = 0;
@@ -240,14 +242,14 @@ __global__ void __launch_bounds__(512, 1) norm_columns_kernel(const __grid_const
             P res[JOIN ? NV : 1];
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                if (FULL || group + k * all < len) {
+                if (FULL || k < count) {
                     h[k] = P::load(a.x + first + k * step);
                     if (JOIN) res[k] = P::load(a.residual + first + k * step);
                 }
             }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                if (FULL || group + k * all < len) {
+                if (FULL || k < count) {
                     if (JOIN) {
                         h[k] = joined<T, V>(h[k], res[k], first + k * step, a.rule, keys);
                         h[k].store(a.sum + first + k * step);
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(512, 1) norm_columns_kernel(const __grid_const
         if (live) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                if (FULL || group + k * all < len) {
+                if (FULL || k < count) {
                     const F f = h[k].floats();
 #pragma unroll
                     for (int i = 0; i < N; ++i) {
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(512, 1) norm_columns_kernel(const __grid_const
         }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            if (FULL || group + k * all < len) {
+            if (FULL || k < count) {
                 const F f = h[k].floats();
                 F out;
 #pragma unroll
@@ -315,7 +317,7 @@ __global__ void __launch_bounds__(512, 1) norm_columns_kernel(const __grid_const
 // A thread adds up its channels' gradients over the tiles that its block (cluster) walks over.  `part` gets
 // [gridDim.x][2][len] sums.
 template <typename T, int V, int NV, bool JOIN, bool FULL>
-__global__ void __launch_bounds__(512, 1) norm_columns_bwd_kernel(const __grid_constant__ NormArgs<T> a) {
+__global__ void __maxnreg__(128) norm_columns_bwd_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
     using F = Floats<V>;
     using E = typename F::E;
@@ -326,7 +328,8 @@ __global__ void __launch_bounds__(512, 1) norm_columns_bwd_kernel(const __grid_c
     const int clusters = gridDim.y, all = groups * clusters;
     const int group = blockIdx.y * groups + threadIdx.y;
     const int len = a.shape.len;
-    const long long step = static_cast<long long>(all) * a.shape.inner;
+    const unsigned step = static_cast<unsigned>(all) * a.shape.inner;  // a sample's elements are counted in 31 bits here
+    const int count = (len - group + all - 1) / all;                    // of this thread's strides
     const float inverse = 1.0f / static_cast<float>(len);
     const bool stores = a.dx != nullptr || (JOIN && a.dropped != nullptr);
     if (JOIN) share_keys(a.rule, keys);
@@ -336,7 +339,7 @@ __global__ void __launch_bounds__(512, 1) norm_columns_bwd_kernel(const __grid_c
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int c = group + k * all;
-        w[k] = (FULL || c < len) && a.weight ? load_param<T>(a.weight, c, a.f32) : 1.0f;
+        w[k] = (FULL || k < count) && a.weight ? load_param<T>(a.weight, c, a.f32) : 1.0f;
         dw[k] = db[k] = splat<E>(0.0f);
     }
 
@@ -353,7 +356,7 @@ __global__ void __launch_bounds__(512, 1) norm_columns_bwd_kernel(const __grid_c
         if (live) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                if (FULL || group + k * all < len) {
+                if (FULL || k < count) {
                     gy[k] = P::load(a.gy + first + k * step);
                     x[k] = P::load(a.x + first + k * step);
                 }
@@ -374,11 +377,11 @@ __global__ void __launch_bounds__(512, 1) norm_columns_bwd_kernel(const __grid_c
             if (JOIN && a.add != nullptr) {
 #pragma unroll
                 for (int k = 0; k < NV; ++k)
-                    if (FULL || group + k * all < len) extra[k] = P::load(a.add + first + k * step);
+                    if (FULL || k < count) extra[k] = P::load(a.add + first + k * step);
             }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                if (FULL || group + k * all < len) {
+                if (FULL || k < count) {
                     const F g = gy[k].floats(), h = x[k].floats();
 #pragma unroll
                     for (int i = 0; i < N; ++i) {
@@ -402,7 +405,7 @@ __global__ void __launch_bounds__(512, 1) norm_columns_bwd_kernel(const __grid_c
             }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                if (FULL || group + k * all < len) {
+                if (FULL || k < count) {
                     const F g = gy[k].floats(), h = x[k].floats();
                     F d;
 #pragma unroll
@@ -427,7 +430,7 @@ __global__ void __launch_bounds__(512, 1) norm_columns_bwd_kernel(const __grid_c
                 float* part = shared + ((k * groups + threadIdx.y) * warps + (lane >> 5)) * 2;
                 part[0] = sw;
                 part[1] = sb;
-            } else if (group + k * all < len) {
+            } else if (k < count) {
                 a.part[(blockIdx.x * 2ll) * len + group + k * all] = sw;
                 a.part[(blockIdx.x * 2ll + 1) * len + group + k * all] = sb;
             }
@@ -436,7 +439,7 @@ __global__ void __launch_bounds__(512, 1) norm_columns_bwd_kernel(const __grid_c
     if (warps > 1) {
         __syncthreads();
         for (int k = lane; k < NV; k += lanes) {
-            if (group + k * all < len) {
+            if (k < count) {
                 const float* part = shared + (k * groups + threadIdx.y) * warps * 2;
                 float sw = 0.0f, sb = 0.0f;
                 for (int i = 0; i < warps; ++i) {
@@ -522,14 +525,15 @@ struct RowPlace {
         all = blockDim.x * gridDim.y;
         first = blockIdx.y * blockDim.x + threadIdx.x;
     }
-    // the row of tile t that is the r-th of this thread's group
-    __device__ __forceinline__ long long row(long long t, int R, int r) const {
-        if (!SHIFTED) return (t * blockDim.y + threadIdx.y) * R + r;
-        return t % V + ((t / V * blockDim.y + threadIdx.y) * R + r) * V;
+    // the first row of tile t that this thread's group takes; the others are kStep apart
+    static constexpr int kStep = SHIFTED ? V : 1;
+    __device__ __forceinline__ long long row(long long t, int R) const {
+        if (!SHIFTED) return (t * blockDim.y + threadIdx.y) * R;
+        return t % V + (t / V * blockDim.y + threadIdx.y) * static_cast<long long>(R * V);
     }
-    // the first element of its vector j in memory
-    __device__ __forceinline__ long long at(long long row, int j) const {
-        return row * len + (static_cast<long long>(j) * V - shift);
+    // the first element of the thread's first vector of a row in memory
+    __device__ __forceinline__ long long at(long long row) const {
+        return row * len + (static_cast<long long>(first) * V - shift);
     }
     __device__ __forceinline__ int lo(int j) const { return SHIFTED && j == 0 ? shift : 0; }
     __device__ __forceinline__ int hi(int j) const {
@@ -547,31 +551,60 @@ struct RowPlace {
         } else if (!SHIFTED) {
             out = load_params<T, V>(p, j * V, f32);
         } else {
-            float f[V];
-            const int first_element = j * V - shift;
+            // aligned groups of a vector's width, from which the vector is cut at `off`, the same place for all threads
+            const int from = j * V - shift, off = (V - shift) % V;
+            float f[2 * V];
+            if (from >= 0 && from - off + 2 * V <= len) {
+                const Floats<V> a = load_params<T, V>(p, from - off, f32), b = load_params<T, V>(p, from - off + V, f32);
+                float parts[V];
+                a.to(parts);
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                f[i] = first_element + i >= 0 && first_element + i < len ? load_param<T>(p, first_element + i, f32) : fill;
-            out.from(f);
+                for (int i = 0; i < V; ++i) f[i] = parts[i];
+                b.to(parts);
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[V + i] = parts[i];
+                // by one, two and four places where off has that bit
+#pragma unroll
+                for (int bit = 1; bit < V; bit *= 2) {
+                    if (off & bit) {
+#pragma unroll
+                        for (int i = 0; i < 2 * V - bit; ++i) f[i] = f[i + bit];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[i] = from + i >= 0 && from + i < len ? load_param<T>(p, from + i, f32) : fill;
+            }
+            float cut[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) cut[i] = f[i];
+            out.from(cut);
         }
         return out;
     }
 };
 
-// The V elements from e on; those that lie before lo or from hi on read as zero where that is asked for (`whole` false).
+// The V elements from e on; of an incomplete vector those before lo and from hi on, another row's, read as zero.
+// `inside`: the whole vector lies in the tensor, which has no more than the last one's end beyond it.
 template <typename T, int V, bool SHIFTED>
-__device__ __forceinline__ Pack<T, V> load_part(const T* p, long long e, bool whole, int lo, int hi) {
+__device__ __forceinline__ Pack<T, V> load_part(const T* p, long long e, bool whole, bool inside, int lo, int hi) {
     if (!SHIFTED || whole) return Pack<T, V>::load(p + e);
     float f[V];
+    if (inside) {
+        Pack<T, V>::load(p + e).floats().to(f);
+    } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = i >= lo && i < hi ? Storage<T>::load(p[e + i]) : 0.0f;
+        for (int i = 0; i < V; ++i) f[i] = i < hi ? Storage<T>::load(p[e + i]) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = i >= lo && i < hi ? f[i] : 0.0f;
     Floats<V> v;
     v.from(f);
     return Pack<T, V>::of(v);
 }
 
 template <typename T, int V, int NV, int R, bool JOIN, bool SHIFTED>
-__global__ void __launch_bounds__(512, 1) norm_rows_kernel(const __grid_constant__ NormArgs<T> a) {
+__global__ void __maxnreg__(JOIN ? 80 : 64) norm_rows_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
     using F = Floats<V>;
     using E = typename F::E;
@@ -581,6 +614,7 @@ __global__ void __launch_bounds__(512, 1) norm_rows_kernel(const __grid_constant
     __shared__ PhiloxKeys keys;
     const RowPlace<V, SHIFTED> place(a.shape);
     const float n = static_cast<float>(place.len), inverse = 1.0f / n;
+    const long long row_step = static_cast<long long>(place.len) * place.kStep;
     if (JOIN) share_keys(a.rule, keys);
     F w[NV], b[NV];
     if (kKeepParams) {
@@ -595,33 +629,33 @@ __global__ void __launch_bounds__(512, 1) norm_rows_kernel(const __grid_constant
     for (long long t = blockIdx.x; t < a.tiles; t += gridDim.x) {
         P h[R][NV];
         float sum[R], squares[R], mean[R], rstd[R];
+        const long long row0 = place.row(t, R), base = place.at(row0);
+        const int rows = static_cast<int>(min((a.shape.rows - row0 + place.kStep - 1) / place.kStep, static_cast<long long>(R)));
         {
             P res[JOIN ? R : 1][NV];
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const long long row = place.row(t, R, r);
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
                     const int j = place.first + k * place.all;
-                    if (row < a.shape.rows && j < place.vectors) {
-                        const long long e = place.at(row, j);
-                        const bool whole = place.whole(j);
-                        h[r][k] = load_part<T, V, SHIFTED>(a.x, e, whole, place.lo(j), place.hi(j));
-                        if (JOIN)
-                            res[r][k] = load_part<T, V, SHIFTED>(a.residual, e, whole, place.lo(j), place.hi(j));
+                    if (r < rows && j < place.vectors) {
+                        const long long e = base + r * row_step + k * place.all * V;
+                        const bool whole = place.whole(j), inside = e + V <= a.shape.rows * place.len;
+                        const int lo = place.lo(j), hi = place.hi(j);
+                        h[r][k] = load_part<T, V, SHIFTED>(a.x, e, whole, inside, lo, hi);
+                        if (JOIN) res[r][k] = load_part<T, V, SHIFTED>(a.residual, e, whole, inside, lo, hi);
                     }
                 }
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const long long row = place.row(t, R, r);
                 E s = splat<E>(0.0f);
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
                     const int j = place.first + k * place.all;
-                    if (row < a.shape.rows && j < place.vectors) {
+                    if (r < rows && j < place.vectors) {
                         if (JOIN) {  // beside the row: dropout and sum of zeros
-                            const long long e = place.at(row, j);
+                            const long long e = base + r * row_step + k * place.all * V;
                             h[r][k] = joined<T, V>(h[r][k], res[r][k], e, a.rule, keys);
                             store_part<T, V>(a.sum + e, h[r][k], place.whole(j), place.lo(j), place.hi(j));
                         }
@@ -641,7 +675,7 @@ __global__ void __launch_bounds__(512, 1) norm_rows_kernel(const __grid_constant
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 const int j = place.first + k * place.all;
-                if (place.row(t, R, r) < a.shape.rows && j < place.vectors) {
+                if (r < rows && j < place.vectors) {
                     F f = h[r][k].floats();
 #pragma unroll
                     for (int i = 0; i < N; ++i) f.e[i] = sub(f.e[i], splat<E>(mean[r]));
@@ -663,10 +697,9 @@ __global__ void __launch_bounds__(512, 1) norm_rows_kernel(const __grid_constant
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             rstd[r] = root_inverse(fmaf(squares[r], inverse, a.eps));
-            const long long row = place.row(t, R, r);
-            if (a.mean != nullptr && place.first == 0 && row < a.shape.rows) {
-                a.mean[row] = mean[r];
-                a.rstd[row] = rstd[r];
+            if (a.mean != nullptr && place.first == 0 && r < rows) {
+                a.mean[row0 + r * place.kStep] = mean[r];
+                a.rstd[row0 + r * place.kStep] = rstd[r];
             }
         }
 #pragma unroll
@@ -677,14 +710,14 @@ __global__ void __launch_bounds__(512, 1) norm_rows_kernel(const __grid_constant
                 const F bk = kKeepParams ? b[k] : place.template params<T>(a.bias, j, a.f32, 0.0f);
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const long long row = place.row(t, R, r);
-                    if (row < a.shape.rows) {
+                    if (r < rows) {
                         const F f = h[r][k].floats();
                         F out;
 #pragma unroll
                         for (int i = 0; i < N; ++i)
                             out.e[i] = fma(mul(sub(f.e[i], splat<E>(mean[r])), splat<E>(rstd[r])), wk.e[i], bk.e[i]);
-                        store_part<T, V>(a.y + place.at(row, j), P::of(out), place.whole(j), place.lo(j), place.hi(j));
+                        store_part<T, V>(a.y + base + r * row_step + k * place.all * V, P::of(out), place.whole(j),
+                                         place.lo(j), place.hi(j));
                     }
                 }
             }
@@ -695,7 +728,7 @@ __global__ void __launch_bounds__(512, 1) norm_rows_kernel(const __grid_constant
 
 // `part` gets [gridDim.x][2][len] sums of the parameters' gradients, one pair per block (cluster).
 template <typename T, int V, int NV, int R, bool JOIN, bool SHIFTED>
-__global__ void __launch_bounds__(NV * V >= 32 ? 256 : 512, 1) norm_rows_bwd_kernel(const __grid_constant__ NormArgs<T> a) {
+__global__ void __maxnreg__(128) norm_rows_bwd_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
     using F = Floats<V>;
     using E = typename F::E;
@@ -706,6 +739,7 @@ __global__ void __launch_bounds__(NV * V >= 32 ? 256 : 512, 1) norm_rows_bwd_ker
     __shared__ PhiloxKeys keys;
     const RowPlace<V, SHIFTED> place(a.shape);
     const float inverse = 1.0f / static_cast<float>(place.len);
+    const long long row_step = static_cast<long long>(place.len) * place.kStep;
     const bool stores = a.dx != nullptr || (JOIN && a.dropped != nullptr);
     if (JOIN) share_keys(a.rule, keys);
 
@@ -721,22 +755,24 @@ __global__ void __launch_bounds__(NV * V >= 32 ? 256 : 512, 1) norm_rows_bwd_ker
     for (long long t = blockIdx.x; t < a.tiles; t += gridDim.x) {
         P gy[R][NV], x[R][NV], extra[JOIN ? R : 1][NV];
         float mean[R], rstd[R], s[2 * R];
+        const long long row0 = place.row(t, R), base = place.at(row0);
+        const int rows = static_cast<int>(min((a.shape.rows - row0 + place.kStep - 1) / place.kStep, static_cast<long long>(R)));
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const long long row = place.row(t, R, r);
-            const bool live = row < a.shape.rows;
-            mean[r] = live ? a.mean[row] : 0.0f;
-            rstd[r] = live ? a.rstd[row] : 0.0f;
+            const bool live = r < rows;
+            mean[r] = live ? a.mean[row0 + r * place.kStep] : 0.0f;
+            rstd[r] = live ? a.rstd[row0 + r * place.kStep] : 0.0f;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 const int j = place.first + k * place.all;
                 if (live && j < place.vectors) {
-                    const long long e = place.at(row, j);
-                    const bool whole = place.whole(j);
+                    const long long e = base + r * row_step + k * place.all * V;
+                    const bool whole = place.whole(j), inside = e + V <= a.shape.rows * place.len;
                     const int lo = place.lo(j), hi = place.hi(j);
-                    gy[r][k] = load_part<T, V, SHIFTED>(a.gy, e, whole, lo, hi);
-                    x[r][k] = load_part<T, V, SHIFTED>(a.x, e, whole, lo, hi);
-                    if (JOIN && a.add != nullptr) extra[r][k] = load_part<T, V, SHIFTED>(a.add, e, whole, lo, hi);
+                    gy[r][k] = load_part<T, V, SHIFTED>(a.gy, e, whole, inside, lo, hi);
+                    x[r][k] = load_part<T, V, SHIFTED>(a.x, e, whole, inside, lo, hi);
+                    if (JOIN && a.add != nullptr)
+                        extra[r][k] = load_part<T, V, SHIFTED>(a.add, e, whole, inside, lo, hi);
                 }
             }
         }
@@ -750,7 +786,7 @@ __global__ void __launch_bounds__(NV * V >= 32 ? 256 : 512, 1) norm_rows_bwd_ker
                 const F wk = kKeepParams ? w[k] : place.template params<T>(a.weight, j, a.f32, 1.0f);
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    if (place.row(t, R, r) < a.shape.rows) {
+                    if (r < rows) {
                         const F g = gy[r][k].floats(), h = x[r][k].floats();
 #pragma unroll
                         for (int i = 0; i < N; ++i) {  // beside the row g is zero
@@ -778,8 +814,7 @@ __global__ void __launch_bounds__(NV * V >= 32 ? 256 : 512, 1) norm_rows_bwd_ker
                     const F wk = kKeepParams ? w[k] : place.template params<T>(a.weight, j, a.f32, 1.0f);
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        const long long row = place.row(t, R, r);
-                        if (row < a.shape.rows) {
+                        if (r < rows) {
                             const E shift = splat<E>(-s[2 * r] * inverse * rstd[r]);
                             const E scale = splat<E>(-s[2 * r + 1] * inverse * (rstd[r] * rstd[r]));
                             const F g = gy[r][k].floats(), h = x[r][k].floats();
@@ -788,8 +823,8 @@ __global__ void __launch_bounds__(NV * V >= 32 ? 256 : 512, 1) norm_rows_bwd_ker
                             for (int i = 0; i < N; ++i)
                                 d.e[i] = fma(mul(g.e[i], wk.e[i]), splat<E>(rstd[r]),
                                              fma(sub(h.e[i], splat<E>(mean[r])), scale, shift));
-                            store_dx<T, V, JOIN>(d, place.at(row, j), a, extra[JOIN ? r : 0][k], keys, place.whole(j),
-                                                 place.lo(j), place.hi(j));
+                            store_dx<T, V, JOIN>(d, base + r * row_step + k * place.all * V, a, extra[JOIN ? r : 0][k],
+                                                 keys, place.whole(j), place.lo(j), place.hi(j));
                         }
                     }
                 }

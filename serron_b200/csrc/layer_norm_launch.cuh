@@ -35,10 +35,13 @@ cudaError_t launch_rows(const NormPlan& p, bool backward, bool join, const NormA
         return launch_norm<T>(
             join ? norm_rows_kernel<T, V, NV, R, true, SHIFTED> : norm_rows_kernel<T, V, NV, R, false, SHIFTED>, p, 0,
             args, stream);
-    const size_t floats = p.ty > 1 ? size_t(NV) * V * p.tx * p.ty : 0;
-    return launch_norm<T>(
-        join ? norm_rows_bwd_kernel<T, V, NV, R, true, SHIFTED> : norm_rows_bwd_kernel<T, V, NV, R, false, SHIFTED>, p,
-        sizeof(float) * floats, args, stream);
+    if constexpr (NV * V <= 16) {
+        const size_t floats = p.ty > 1 ? size_t(NV) * V * p.tx * p.ty : 0;
+        return launch_norm<T>(
+            join ? norm_rows_bwd_kernel<T, V, NV, R, true, SHIFTED> : norm_rows_bwd_kernel<T, V, NV, R, false, SHIFTED>,
+            p, sizeof(float) * floats, args, stream);
+    }
+    return cudaErrorInvalidConfiguration;
 }
 
 template <typename T, int V, int NV, bool FULL>

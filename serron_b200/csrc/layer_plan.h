@@ -36,25 +36,24 @@ inline void plan_rows(NormPlan& p, int64_t rows, int64_t len, int size, bool bac
     const bool wide = p.V * size == 16;
     p.shifted = len % p.V != 0;
     const int64_t vectors = plan_ceil(len + (p.shifted ? p.V - 1 : 0), p.V);
-    // the sums for the parameters' gradients of 32 elements a thread leave room for half as many threads
-    const auto most_threads = [&](int nv) { return backward && nv * p.V >= 32 ? 256 : 512; };
-    // a row to one warp where 32 elements a thread are enough (16 where V does not divide len: the parameters
-    // then stay in registers), else to as few warps as may be: what is done once a row and thread is shared by more elements
-    p.NV = wide ? (vectors <= 32 ? 1 : vectors <= 64 || (p.shifted && vectors <= 1024) ? 2 : 4) : (vectors <= 128 ? 4 : 16);
+    constexpr int kMostThreads = 512;
+    // a row to as few warps as may be, so that what is done once a row and thread is shared by more elements; a backward
+    // pass also keeps two sums for each of a thread's elements of a row, and takes no more than 16
+    const int most = wide ? (backward && p.V == 8 ? 2 : 4) : 16;
+    p.NV = wide ? (vectors <= 32 ? 1 : vectors <= 64 ? 2 : most) : (vectors <= 128 ? 4 : 16);
     p.R = wide ? 4 / p.NV : p.NV == 4 ? 4 : 1;
     int64_t threads = plan_ceil(vectors, p.NV);
     // few rows: one at a time, with fewer vectors per thread and over more blocks
-    if (plan_ceil(rows, p.R) * std::max<int64_t>(threads, 32) < int64_t(kSMs) * 256) {
+    if (plan_ceil(rows, p.R) * std::max<int64_t>(threads, 32) < int64_t(kSMs) * 512) {
         p.R = 1;
-        const int most = wide ? 4 : 16;
         p.NV = wide ? 1 : 4;
         while (p.NV < most && plan_ceil(vectors, p.NV) > (rows < kSMs ? 4 : 1) * 512) p.NV = wide ? 2 * p.NV : 16;
         threads = plan_ceil(vectors, p.NV);
         while (p.clusters < 8 && rows * p.clusters < kSMs && threads > 256 * p.clusters) p.clusters *= 2;
     }
-    while (p.clusters < 8 && threads > int64_t(most_threads(p.NV)) * p.clusters) p.clusters *= 2;
+    while (p.clusters < 8 && threads > int64_t(kMostThreads) * p.clusters) p.clusters *= 2;
     threads = plan_ceil(threads, p.clusters);
-    if (threads > most_threads(p.NV)) return;
+    if (threads > kMostThreads) return;
     if (threads <= 32) {
         p.tx = 1;
         while (p.tx < threads) p.tx *= 2;
@@ -71,8 +70,9 @@ inline void plan_rows(NormPlan& p, int64_t rows, int64_t len, int size, bool bac
 }
 
 // Columns: NV = 4, 8 (and 16 for 16-bit forward passes) with V = 4, NV = 8, 16 with V = 1.
-inline void plan_columns(NormPlan& p, int64_t rows, int64_t len, int size, bool backward) {
+inline void plan_columns(NormPlan& p, int64_t rows, int64_t len, int64_t inner, int size, bool backward) {
     const int64_t columns = rows / p.V;
+    if (len * inner >= int64_t(1) << 31) return;
     // what fits in registers without spilling: 64 bytes of each tensor, of the one of a forward pass 128
     int per = p.V == 4 ? (backward ? 8 : 16) / (size / 2) : 16;
     if (p.V == 4) per = std::max(per, 4);
@@ -100,20 +100,17 @@ inline NormPlan norm_plan(int64_t rows, int64_t len, int64_t inner, int V, int s
     if (p.rows)
         plan_rows(p, rows, len, size, backward);
     else
-        plan_columns(p, rows, len, size, backward);
+        plan_columns(p, rows, len, inner, size, backward);
     if (!p.ok) return p;
+    // the grid walks over the tiles: as many blocks as are resident, each with the same number of tiles (or one, where that is
+    // two rounds of blocks at most)
     const int threads = p.tx * p.ty;
-    int64_t each;
-    if (backward) {
-        // as many blocks as are resident, each with the same number of tiles, and no more than 128 rows to a sum of the
-        // parameters' gradients, which keeps those as exact as a tree's
-        const int on_an_sm = p.rows && p.NV * p.V >= 32 ? 384 : 512;
-        const int64_t resident = std::max<int64_t>(1, int64_t(kSMs) * std::max(1, on_an_sm / threads) / p.clusters);
-        each = std::min<int64_t>(plan_ceil(p.tiles, resident), 128 / p.R);
-    } else {
-        // what a block does once is shared by a few tiles where there are many
-        each = std::min<int64_t>(8, std::max<int64_t>(1, p.tiles * threads * p.clusters / (int64_t(kSMs) * 4096)));
-    }
+    const int64_t resident = std::max<int64_t>(1, int64_t(kSMs) * std::max(1, 512 / threads) / p.clusters);
+    int64_t each = p.tiles <= 2 * resident ? 1 : plan_ceil(p.tiles, resident);
+    if (backward)  // no more than 128 rows to a sum of the parameters' gradients, which keeps those as exact as a tree's
+        each = std::min<int64_t>(each, 128 / p.R);
+    else  // blocks that end early make room for others
+        each = std::min<int64_t>(each, 8);
     p.blocks = plan_ceil(p.tiles, each);
     // a block of shifted rows takes every V-th tile
     if (p.shifted && p.blocks < p.tiles) p.blocks = std::min(p.tiles, plan_ceil(p.blocks, p.V) * p.V);
