@@ -224,6 +224,29 @@ __global__ void __launch_bounds__(kNormThreads)
     part[(block * 2 + 1) * s.len + l] = db;
 }
 
+// inner == 1 and few rows: a thread owns an element of the row, and what it adds up is the gradient.
+template <typename T>
+__global__ void __launch_bounds__(128)
+    norm_param_direct_kernel(const T* __restrict__ gy, const T* __restrict__ x,
+                             const typename Storage<T>::acc* __restrict__ mean,
+                             const typename Storage<T>::acc* __restrict__ rstd, void* __restrict__ dw,
+                             void* __restrict__ db, bool f32, NormShape s) {
+    using S = Storage<T>;
+    using A = typename S::acc;
+    const int l = blockIdx.x * 128 + threadIdx.x;
+    if (l >= s.len) return;
+    A w = A(0), b = A(0);
+#pragma unroll 8
+    for (int r = 0; r < static_cast<int>(s.rows); ++r) {
+        const long long e = static_cast<long long>(r) * s.len + l;
+        const A g = S::load(gy[e]);
+        w += g * ((S::load(x[e]) - mean[r]) * rstd[r]);
+        b += g;
+    }
+    if (dw) store_param<T>(dw, l, f32, w);
+    if (db) store_param<T>(db, l, f32, b);
+}
+
 // inner > 1: a block sums rows_per neighbouring rows at one element of them.
 template <typename T>
 __global__ void __launch_bounds__(kNormThreads)

@@ -604,7 +604,7 @@ __device__ __forceinline__ Pack<T, V> load_part(const T* p, long long e, bool wh
 }
 
 template <typename T, int V, int NV, int R, bool JOIN, bool SHIFTED>
-__global__ void __maxnreg__(JOIN ? 80 : 64) norm_rows_kernel(const __grid_constant__ NormArgs<T> a) {
+__global__ void __maxnreg__((JOIN ? 80 : 64) + (SHIFTED ? 32 : 0)) norm_rows_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
     using F = Floats<V>;
     using E = typename F::E;

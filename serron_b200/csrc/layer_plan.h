@@ -51,7 +51,7 @@ inline void plan_rows(NormPlan& p, int64_t rows, int64_t len, int size, bool bac
         threads = plan_ceil(vectors, p.NV);
         while (p.clusters < 8 && rows * p.clusters < kSMs && threads > 256 * p.clusters) p.clusters *= 2;
     }
-    while (p.clusters < 8 && threads > int64_t(kMostThreads) * p.clusters) p.clusters *= 2;
+    while (p.clusters < 8 && threads > 256 * p.clusters) p.clusters *= 2;  // several blocks to an SM
     threads = plan_ceil(threads, p.clusters);
     if (threads > kMostThreads) return;
     if (threads <= 32) {
@@ -71,11 +71,10 @@ inline void plan_rows(NormPlan& p, int64_t rows, int64_t len, int size, bool bac
 
 // Columns: NV = 4, 8 (and 16 for 16-bit forward passes) with V = 4, NV = 8, 16 with V = 1.
 inline void plan_columns(NormPlan& p, int64_t rows, int64_t len, int64_t inner, int size, bool backward) {
-    const int64_t columns = rows / p.V;
     if (len * inner >= int64_t(1) << 31) return;
+    const int64_t columns = rows / p.V;
     // what fits in registers without spilling: 64 bytes of each tensor, of the one of a forward pass 128
-    int per = p.V == 4 ? (backward ? 8 : 16) / (size / 2) : 16;
-    if (p.V == 4) per = std::max(per, 4);
+    int per = p.V == 4 ? std::max(4, (backward ? 8 : 16) / (size / 2)) : 16;
     const int least = p.V == 4 ? 4 : 8;
     while (per > least && (len <= per / 2 || columns * plan_ceil(len, per) < int64_t(kSMs) * 512) &&
            plan_ceil(len, per / 2) <= 16)
@@ -105,12 +104,13 @@ inline NormPlan norm_plan(int64_t rows, int64_t len, int64_t inner, int V, int s
     // the grid walks over the tiles: as many blocks as are resident, each with the same number of tiles (or one, where that is
     // two rounds of blocks at most)
     const int threads = p.tx * p.ty;
-    const int64_t resident = std::max<int64_t>(1, int64_t(kSMs) * std::max(1, 512 / threads) / p.clusters);
+    const int on_an_sm = p.rows && !backward ? 1024 : 512;
+    const int64_t resident = std::max<int64_t>(1, int64_t(kSMs) * std::max(1, on_an_sm / threads) / p.clusters);
     int64_t each = p.tiles <= 2 * resident ? 1 : plan_ceil(p.tiles, resident);
     if (backward)  // no more than 128 rows to a sum of the parameters' gradients, which keeps those as exact as a tree's
         each = std::min<int64_t>(each, 128 / p.R);
-    else  // blocks that end early make room for others
-        each = std::min<int64_t>(each, 8);
+    else if (p.rows)  // little is done once a block: rather four rounds of blocks
+        each = std::max<int64_t>(1, each / 4);
     p.blocks = plan_ceil(p.tiles, each);
     // a block of shifted rows takes every V-th tile
     if (p.shifted && p.blocks < p.tiles) p.blocks = std::min(p.tiles, plan_ceil(p.blocks, p.V) * p.V);

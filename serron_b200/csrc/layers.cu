@@ -122,6 +122,8 @@ struct Norm {
 // Rows per first-level sum of the parameters' gradients: at most 128 additions in a row (32 per thread where a
 // block's threads share a sum), so that the float32 sums stay as exact as a tree's.
 constexpr int kRowsPerSum = 128, kColumnsPerSum = 32 * kNormThreads;
+// Up to so many rows the gradients of weight and bias are added up straight from the tensors.
+constexpr int kDirectRows = 64;
 
 Norm norm_of(const char* name, int64_t outer, int64_t len, int64_t inner) {
     SB_CHECK(outer >= 0 && inner >= 0, name, ": sizes must be non-negative");
@@ -260,6 +262,8 @@ void norm_backward(const char* name, const Norm& n, const void* gy_, const void*
                    const void* rstd_, const void* weight, bool f32, const void* add, const DropRule& rule, void* dx,
                    void* dropped, void* dw, void* db, char* ws, cudaStream_t stream, bool join) {
     using A = typename Storage<T>::acc;
+    const T *gy = static_cast<const T*>(gy_), *x = static_cast<const T*>(x_);
+    const A *mean = static_cast<const A*>(mean_), *rstd = static_cast<const A*>(rstd_);
     if constexpr (!std::is_same_v<T, double>) {
         const NormPlan p = n.plan(dtype_of<T>, true, [&](int v) {
             return fits(v * sizeof(T), gy_, x_, add, dx, dropped) && params_fit<T>(v, f32, weight);
@@ -275,19 +279,25 @@ void norm_backward(const char* name, const Norm& n, const void* gy_, const void*
             a.add = static_cast<const T*>(add);
             a.dx = static_cast<T*>(dx);
             a.dropped = static_cast<T*>(dropped);
-            a.part = dw || db ? reinterpret_cast<float*>(ws) : nullptr;
+            // few rows: their partial sums would be as large as the tensors, which are read again instead
+            const bool direct = p.rows && n.shape.rows <= kDirectRows;
+            a.part = (dw || db) && !direct ? reinterpret_cast<float*>(ws) : nullptr;
             a.shape = n.shape;
             a.rule = rule;
             a.stats_wide = fits(sizeof(float) * p.V, a.mean, a.rstd);
             a.tiles = p.tiles;
-            SB_CUDA(norm_launch<T>(p, true, join, a, stream));
-            if (dw || db) param_final<T>(a.part, p.blocks, n.shape.len, dw, db, f32, stream);
+            if (!direct || dx || dropped) SB_CUDA(norm_launch<T>(p, true, join, a, stream));
+            if (a.part) {
+                param_final<T>(a.part, p.blocks, n.shape.len, dw, db, f32, stream);
+            } else if (dw || db) {
+                norm_param_direct_kernel<T><<<ceil_div(n.shape.len, 128), 128, 0, stream>>>(gy, x, mean, rstd, dw, db,
+                                                                                            f32, n.shape);
+                SB_CUDA(cudaGetLastError());
+            }
             return;
         }
     }
     const NormWorkspace w(n, sizeof(A), true);
-    const T *gy = static_cast<const T*>(gy_), *x = static_cast<const T*>(x_);
-    const A *mean = static_cast<const A*>(mean_), *rstd = static_cast<const A*>(rstd_);
     A* part = reinterpret_cast<A*>(ws + w.part);
     A* sums = reinterpret_cast<A*>(ws + w.params);
     const bool rows = n.shape.inner == 1;
