@@ -4,6 +4,6 @@
 
 namespace serron {
 
-template cudaError_t norm_launch<__nv_bfloat16>(const NormPlan&, bool, bool, const NormArgs<__nv_bfloat16>&, cudaStream_t);
+template cudaError_t norm_launch<__nv_bfloat16>(const NormPlan&, bool, int, const NormArgs<__nv_bfloat16>&, cudaStream_t);
 
 }  // namespace serron

@@ -4,6 +4,6 @@
 
 namespace serron {
 
-template cudaError_t norm_launch<__half>(const NormPlan&, bool, bool, const NormArgs<__half>&, cudaStream_t);
+template cudaError_t norm_launch<__half>(const NormPlan&, bool, int, const NormArgs<__half>&, cudaStream_t);
 
 }  // namespace serron

@@ -4,6 +4,6 @@
 
 namespace serron {
 
-template cudaError_t norm_launch<float>(const NormPlan&, bool, bool, const NormArgs<float>&, cudaStream_t);
+template cudaError_t norm_launch<float>(const NormPlan&, bool, int, const NormArgs<float>&, cudaStream_t);
 
 }  // namespace serron

@@ -65,16 +65,21 @@ __device__ __forceinline__ float root_inverse(float v) {
     return v < __int_as_float(0x7f800000) ? better : r;
 }
 
-// The generator's keys, in shared memory: a launch takes its seed from the host or from device memory.
-__device__ __forceinline__ void share_keys(const DropRule& rule, PhiloxKeys& shared) {
+// What the kernels are compiled for: the norm alone, or the join with its seed from the host (the generator's keys are operands in
+// constant memory) or in device memory (in shared memory).
+enum Join : int { kNoJoin = 0, kHostSeed = 1, kDeviceSeed = 2 };
+
+template <int JOIN>
+__device__ __forceinline__ const PhiloxKeys& join_keys(const DropRule& rule, PhiloxKeys& shared) {
+    if (JOIN != kDeviceSeed) return rule.keys;
     const int r = threadIdx.y * blockDim.x + threadIdx.x;
     if (r < kPhiloxRounds) {
-        const uint64_t seed = rule.seed_device ? __ldg(rule.seed_device) : 0;
-        shared.k[2 * r] = rule.seed_device ? static_cast<uint32_t>(seed) + r * kPhiloxKey0 : rule.keys.k[2 * r];
-        shared.k[2 * r + 1] =
-            rule.seed_device ? static_cast<uint32_t>(seed >> 32) + r * kPhiloxKey1 : rule.keys.k[2 * r + 1];
+        const uint64_t seed = __ldg(rule.seed_device);
+        shared.k[2 * r] = static_cast<uint32_t>(seed) + r * kPhiloxKey0;
+        shared.k[2 * r + 1] = static_cast<uint32_t>(seed >> 32) + r * kPhiloxKey1;
     }
     __syncthreads();
+    return shared;
 }
 
 // dropout(v) for the elements from e on.
@@ -117,7 +122,7 @@ __device__ __forceinline__ void store_part(T* p, const Pack<T, V>& v, bool whole
 }
 
 // What follows dx = v from element e on: the sum with `extra`, dx itself, and its masked copy.
-template <typename T, int V, bool JOIN>
+template <typename T, int V, int JOIN>
 __device__ __forceinline__ void store_dx(Floats<V> v, long long e, const NormArgs<T>& a, const Pack<T, V>& extra,
                                          const PhiloxKeys& keys, bool whole = true, int lo = 0, int hi = V) {
     if (JOIN && a.add != nullptr) {
@@ -203,14 +208,14 @@ __device__ __forceinline__ void column_totals(Floats<V> (&v)[M], float* shared, 
 }
 
 // FULL: every thread has all of its NV strides (len is their number times the groups').
-template <typename T, int V, int NV, bool JOIN, bool FULL>
+template <typename T, int V, int NV, int JOIN, bool FULL>
 __global__ void __maxnreg__(JOIN ? 128 : 96) norm_columns_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
     using F = Floats<V>;
     using E = typename F::E;
     constexpr int N = F::N;
     extern __shared__ __align__(16) float shared[];
-    __shared__ PhiloxKeys keys;
+    __shared__ PhiloxKeys own_keys;
     const int lanes = blockDim.x, lane = threadIdx.x;
     const int clusters = gridDim.y, all = blockDim.y * clusters;
     const int group = blockIdx.y * blockDim.y + threadIdx.y;
@@ -218,7 +223,7 @@ __global__ void __maxnreg__(JOIN ? 128 : 96) norm_columns_kernel(const __grid_co
     const unsigned step = static_cast<unsigned>(all) * a.shape.inner;  // a sample's elements are counted in 31 bits here
     const int count = (len - group + all - 1) / all;                    // of this thread's strides
     const float n = static_cast<float>(len), inverse = 1.0f / n;
-    if (JOIN) share_keys(a.rule, keys);
+    const PhiloxKeys& keys = join_keys<JOIN>(a.rule, own_keys);
 
     float w[NV], b[NV];
 #pragma unroll
@@ -316,14 +321,14 @@ __global__ void __maxnreg__(JOIN ? 128 : 96) norm_columns_kernel(const __grid_co
 
 // A thread adds up its channels' gradients over the tiles that its block (cluster) walks over.  `part` gets
 // [gridDim.x][2][len] sums.
-template <typename T, int V, int NV, bool JOIN, bool FULL>
+template <typename T, int V, int NV, int JOIN, bool FULL>
 __global__ void __maxnreg__(128) norm_columns_bwd_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
     using F = Floats<V>;
     using E = typename F::E;
     constexpr int N = F::N;
     extern __shared__ __align__(16) float shared[];  // column_totals'; at the end two floats a channel and warp
-    __shared__ PhiloxKeys keys;
+    __shared__ PhiloxKeys own_keys;
     const int lanes = blockDim.x, groups = blockDim.y, lane = threadIdx.x;
     const int clusters = gridDim.y, all = groups * clusters;
     const int group = blockIdx.y * groups + threadIdx.y;
@@ -332,7 +337,7 @@ __global__ void __maxnreg__(128) norm_columns_bwd_kernel(const __grid_constant__
     const int count = (len - group + all - 1) / all;                    // of this thread's strides
     const float inverse = 1.0f / static_cast<float>(len);
     const bool stores = a.dx != nullptr || (JOIN && a.dropped != nullptr);
-    if (JOIN) share_keys(a.rule, keys);
+    const PhiloxKeys& keys = join_keys<JOIN>(a.rule, own_keys);
 
     float w[NV];
     E dw[NV], db[NV];
@@ -603,7 +608,7 @@ __device__ __forceinline__ Pack<T, V> load_part(const T* p, long long e, bool wh
     return Pack<T, V>::of(v);
 }
 
-template <typename T, int V, int NV, int R, bool JOIN, bool SHIFTED>
+template <typename T, int V, int NV, int R, int JOIN, bool SHIFTED>
 __global__ void __maxnreg__((JOIN ? 80 : 64) + (SHIFTED ? 32 : 0)) norm_rows_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
     using F = Floats<V>;
@@ -611,11 +616,11 @@ __global__ void __maxnreg__((JOIN ? 80 : 64) + (SHIFTED ? 32 : 0)) norm_rows_ker
     constexpr int N = F::N;
     constexpr bool kKeepParams = SHIFTED && NV <= 2;  // unaligned parameters are read once
     __shared__ RowScratch<R> scratch;
-    __shared__ PhiloxKeys keys;
+    __shared__ PhiloxKeys own_keys;
     const RowPlace<V, SHIFTED> place(a.shape);
     const float n = static_cast<float>(place.len), inverse = 1.0f / n;
     const long long row_step = static_cast<long long>(place.len) * place.kStep;
-    if (JOIN) share_keys(a.rule, keys);
+    const PhiloxKeys& keys = join_keys<JOIN>(a.rule, own_keys);
     F w[NV], b[NV];
     if (kKeepParams) {
 #pragma unroll
@@ -727,7 +732,7 @@ __global__ void __maxnreg__((JOIN ? 80 : 64) + (SHIFTED ? 32 : 0)) norm_rows_ker
 }
 
 // `part` gets [gridDim.x][2][len] sums of the parameters' gradients, one pair per block (cluster).
-template <typename T, int V, int NV, int R, bool JOIN, bool SHIFTED>
+template <typename T, int V, int NV, int R, int JOIN, bool SHIFTED>
 __global__ void __maxnreg__(128) norm_rows_bwd_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
     using F = Floats<V>;
@@ -736,12 +741,12 @@ __global__ void __maxnreg__(128) norm_rows_bwd_kernel(const __grid_constant__ No
     constexpr bool kKeepParams = SHIFTED && NV <= 2;
     __shared__ RowScratch<2 * R> scratch;
     extern __shared__ __align__(16) float sums[];  // [NV][V][threads] where a block has several groups
-    __shared__ PhiloxKeys keys;
+    __shared__ PhiloxKeys own_keys;
     const RowPlace<V, SHIFTED> place(a.shape);
     const float inverse = 1.0f / static_cast<float>(place.len);
     const long long row_step = static_cast<long long>(place.len) * place.kStep;
     const bool stores = a.dx != nullptr || (JOIN && a.dropped != nullptr);
-    if (JOIN) share_keys(a.rule, keys);
+    const PhiloxKeys& keys = join_keys<JOIN>(a.rule, own_keys);
 
     F dw[NV], db[NV], w[NV];
 #pragma unroll

@@ -96,6 +96,7 @@ inline NormPlan norm_plan(int64_t rows, int64_t len, int64_t inner, int V, int s
     p.rows = inner == 1;
     p.V = V;
     if (rows == 0 || (!p.rows && inner % V != 0)) return p;
+    if (rows > (int64_t(1) << 34) / len) return p;  // the join's generator counts blocks of four elements in 32 bits here
     if (p.rows)
         plan_rows(p, rows, len, size, backward);
     else

@@ -210,20 +210,20 @@ __device__ __forceinline__ Floats<V> load_params(const void* p, int i, bool f32)
     }
 }
 
-// The words of decisions e .. e + V - 1, where e is a multiple of min(V, 4).
+// The words of decisions e .. e + V - 1, where e is a multiple of min(V, 4) and below 2^34.
 template <int V>
 __device__ __forceinline__ void drop_words(long long e, uint64_t sequence, const PhiloxKeys& keys, uint32_t (&out)[V]) {
     if constexpr (V >= 4) {
 #pragma unroll
         for (int k = 0; k < V; k += 4) {
-            const uint4 w = philox((e >> 2) + k / 4, sequence, keys);
+            const uint4 w = philox(static_cast<uint32_t>(e >> 2) + k / 4, 0u, sequence, keys);
             out[k] = w.x;
             out[k + 1] = w.y;
             out[k + 2] = w.z;
             out[k + 3] = w.w;
         }
     } else {
-        const uint4 w = philox(e >> 2, sequence, keys);
+        const uint4 w = philox(static_cast<uint32_t>(e >> 2), 0u, sequence, keys);
         if constexpr (V == 2) {
             out[0] = e & 2 ? w.z : w.x;
             out[1] = e & 2 ? w.w : w.y;

@@ -16,7 +16,7 @@ namespace serron {
 
 // the register kernels, instantiated per storage type in layer_norm_<type>.cu
 template <typename T>
-cudaError_t norm_launch(const NormPlan& p, bool backward, bool join, const NormArgs<T>& args, cudaStream_t stream);
+cudaError_t norm_launch(const NormPlan& p, bool backward, int join, const NormArgs<T>& args, cudaStream_t stream);
 
 namespace {
 
@@ -182,6 +182,10 @@ constexpr int dtype_of = std::is_same_v<T, float>    ? kF32
                          : std::is_same_v<T, double> ? kF64
                                                      : kBF16;
 
+int join_kind(bool join, const DropRule& rule) {
+    return !join ? kNoJoin : rule.seed_device ? kDeviceSeed : kHostSeed;
+}
+
 // Every pointer on a boundary of `bytes` (null ones are).
 template <typename... P>
 bool fits(size_t bytes, P... pointers) {
@@ -231,7 +235,7 @@ void norm_forward(const char* name, const Norm& n, const void* x_, const void* w
             a.rule = rule;
             a.stats_wide = fits(sizeof(float) * p.V, a.mean, a.rstd);
             a.tiles = p.tiles;
-            SB_CUDA(norm_launch<T>(p, false, join, a, stream));
+            SB_CUDA(norm_launch<T>(p, false, join_kind(join, rule), a, stream));
             return;
         }
     }
@@ -286,7 +290,7 @@ void norm_backward(const char* name, const Norm& n, const void* gy_, const void*
             a.rule = rule;
             a.stats_wide = fits(sizeof(float) * p.V, a.mean, a.rstd);
             a.tiles = p.tiles;
-            if (!direct || dx || dropped) SB_CUDA(norm_launch<T>(p, true, join, a, stream));
+            if (!direct || dx || dropped) SB_CUDA(norm_launch<T>(p, true, join_kind(join, rule), a, stream));
             if (a.part) {
                 param_final<T>(a.part, p.blocks, n.shape.len, dw, db, f32, stream);
             } else if (dw || db) {

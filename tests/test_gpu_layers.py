@@ -439,6 +439,19 @@ def test_join_maps(serron, shape, dtype):
     _check_join(serron, shape, 1, dtype, 0.3, "f32" if shape[1] % 2 else "same", sum(shape))
 
 
+@pytest.mark.parametrize("shape", [(12, 96), (3, 1001), (2, 10, 6, 6), (2, 10, 5, 5), (1, 3000, 3, 3)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_join_with_its_seed_in_a_tensor(serron, shape, dtype):
+    x, r, gy, gh = (_rand(shape, dtype, k) for k in range(4))
+    leaves = [x.requires_grad_(), r.requires_grad_()]
+    out = []
+    for seed in (77, torch.tensor(77, device="cuda")):
+        y, h = serron.dropout_add_layer_norm(x, r, p=0.3, seed=seed, sequence=5)
+        out.append([y, h, *torch.autograd.grad((y, h), leaves, (gy, gh))])
+    for a, c in zip(*out):
+        assert torch.equal(a, c)
+
+
 @pytest.mark.parametrize("p", [0.0, 0.5, 1.0])
 @pytest.mark.parametrize("params", ["none", "weight", "bias", "f32"])
 def test_join_probabilities_and_params(serron, p, params):
