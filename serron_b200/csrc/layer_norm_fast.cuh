@@ -65,16 +65,19 @@ __device__ __forceinline__ float root_inverse(float v) {
     return v < __int_as_float(0x7f800000) ? better : r;
 }
 
-// What the kernels are compiled for: the norm alone, or the join with its seed from the host (the generator's keys are operands in
-// constant memory) or in device memory (in shared memory).
-enum Join : int { kNoJoin = 0, kHostSeed = 1, kDeviceSeed = 2 };
+// What the kernels are compiled for: the norm alone, or the join with the generator's keys as operands in constant memory
+// (a seed from the host) or in shared memory (any seed).  The backward pass of columns always has them in shared memory: beside its
+// other registers, operands made it slower (378 us against 360 at (64,32,256,256) bfloat16).
+enum Join : int { kNoJoin = 0, kHostSeed = 1, kAnySeed = 2 };
 
 template <int JOIN>
 __device__ __forceinline__ const PhiloxKeys& join_keys(const DropRule& rule, PhiloxKeys& shared) {
-    if (JOIN != kDeviceSeed) return rule.keys;
+    if (JOIN != kAnySeed) return rule.keys;
     const int r = threadIdx.y * blockDim.x + threadIdx.x;
     if (r < kPhiloxRounds) {
-        const uint64_t seed = __ldg(rule.seed_device);
+        // the first round's keys are the seed
+        const uint64_t seed = rule.seed_device ? __ldg(rule.seed_device)
+                                               : rule.keys.k[0] | static_cast<uint64_t>(rule.keys.k[1]) << 32;
         shared.k[2 * r] = static_cast<uint32_t>(seed) + r * kPhiloxKey0;
         shared.k[2 * r + 1] = static_cast<uint32_t>(seed >> 32) + r * kPhiloxKey1;
     }

@@ -31,23 +31,24 @@ cudaError_t launch_norm(void (*kernel)(NormArgs<T>), const NormPlan& p, size_t s
 
 // The kernel for `join` of the three.
 template <typename T>
-auto join_kernel(int join, void (*none)(NormArgs<T>), void (*host)(NormArgs<T>), void (*device)(NormArgs<T>)) {
-    return join == kNoJoin ? none : join == kHostSeed ? host : device;
+auto of_join(int join, void (*none)(NormArgs<T>), void (*host)(NormArgs<T>), void (*any)(NormArgs<T>)) {
+    return join == kNoJoin ? none : join == kHostSeed ? host : any;
 }
 
 template <typename T, int V, int NV, int R, bool SHIFTED>
 cudaError_t launch_rows(const NormPlan& p, bool backward, int join, const NormArgs<T>& args, cudaStream_t stream) {
-    if (!backward)
-        return launch_norm<T>(
-            join_kernel<T>(join, norm_rows_kernel<T, V, NV, R, kNoJoin, SHIFTED>, norm_rows_kernel<T, V, NV, R, kHostSeed, SHIFTED>,
-                       norm_rows_kernel<T, V, NV, R, kDeviceSeed, SHIFTED>), p, 0,
-            args, stream);
+    if (!backward) {
+        auto kernel = of_join<T>(join, norm_rows_kernel<T, V, NV, R, kNoJoin, SHIFTED>,
+                                 norm_rows_kernel<T, V, NV, R, kHostSeed, SHIFTED>,
+                                 norm_rows_kernel<T, V, NV, R, kAnySeed, SHIFTED>);
+        return launch_norm<T>(kernel, p, 0, args, stream);
+    }
     if constexpr (NV * V <= 16) {
+        auto kernel = of_join<T>(join, norm_rows_bwd_kernel<T, V, NV, R, kNoJoin, SHIFTED>,
+                                 norm_rows_bwd_kernel<T, V, NV, R, kHostSeed, SHIFTED>,
+                                 norm_rows_bwd_kernel<T, V, NV, R, kAnySeed, SHIFTED>);
         const size_t floats = p.ty > 1 ? size_t(NV) * V * p.tx * p.ty : 0;
-        return launch_norm<T>(
-            join_kernel<T>(join, norm_rows_bwd_kernel<T, V, NV, R, kNoJoin, SHIFTED>, norm_rows_bwd_kernel<T, V, NV, R, kHostSeed, SHIFTED>,
-                       norm_rows_bwd_kernel<T, V, NV, R, kDeviceSeed, SHIFTED>),
-            p, sizeof(float) * floats, args, stream);
+        return launch_norm<T>(kernel, p, sizeof(float) * floats, args, stream);
     }
     return cudaErrorInvalidConfiguration;
 }
@@ -56,18 +57,18 @@ template <typename T, int V, int NV, bool FULL>
 cudaError_t launch_columns(const NormPlan& p, bool backward, int join, const NormArgs<T>& args, cudaStream_t stream) {
     // column_totals' scratch for one number a row, for two in a backward pass
     const size_t floats = (p.ty > 1 || p.clusters > 1) ? (2 * size_t(p.ty) + 2) * p.tx * V : 0;
-    if (!backward)
-        return launch_norm<T>(
-            join_kernel<T>(join, norm_columns_kernel<T, V, NV, kNoJoin, FULL>, norm_columns_kernel<T, V, NV, kHostSeed, FULL>,
-                       norm_columns_kernel<T, V, NV, kDeviceSeed, FULL>), p,
-            sizeof(float) * floats, args, stream);
+    if (!backward) {
+        auto kernel = of_join<T>(join, norm_columns_kernel<T, V, NV, kNoJoin, FULL>,
+                                 norm_columns_kernel<T, V, NV, kHostSeed, FULL>,
+                                 norm_columns_kernel<T, V, NV, kAnySeed, FULL>);
+        return launch_norm<T>(kernel, p, sizeof(float) * floats, args, stream);
+    }
     if constexpr (NV * V * sizeof(T) <= 64) {
+        auto kernel = join == kNoJoin ? norm_columns_bwd_kernel<T, V, NV, kNoJoin, FULL>
+                                      : norm_columns_bwd_kernel<T, V, NV, kAnySeed, FULL>;
         // at the end two sums per channel and warp
         const size_t most = std::max(2 * floats, size_t(NV) * p.ty * (p.tx / 32) * 2);
-        return launch_norm<T>(
-            join_kernel<T>(join, norm_columns_bwd_kernel<T, V, NV, kNoJoin, FULL>, norm_columns_bwd_kernel<T, V, NV, kHostSeed, FULL>,
-                       norm_columns_bwd_kernel<T, V, NV, kDeviceSeed, FULL>), p,
-            sizeof(float) * most, args, stream);
+        return launch_norm<T>(kernel, p, sizeof(float) * most, args, stream);
     }
     return cudaErrorInvalidConfiguration;
 }

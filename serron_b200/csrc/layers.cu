@@ -183,7 +183,7 @@ constexpr int dtype_of = std::is_same_v<T, float>    ? kF32
                                                      : kBF16;
 
 int join_kind(bool join, const DropRule& rule) {
-    return !join ? kNoJoin : rule.seed_device ? kDeviceSeed : kHostSeed;
+    return !join ? kNoJoin : rule.seed_device ? kAnySeed : kHostSeed;
 }
 
 // Every pointer on a boundary of `bytes` (null ones are).
