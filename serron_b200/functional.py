@@ -166,9 +166,9 @@ def dropout(input_: torch.Tensor, p: float = 0.5, *, seed: int | torch.Tensor, s
     rule = _layer_ops.check_drop("dropout", input_, p, seed, sequence)
     if residual is not None:
         _layer_ops.check_residual("dropout", input_, residual)
-    span = 1
+    span, unit = 1, DropoutUnit(unit)
     if unit is not DropoutUnit.ELEMENT:
-        lead = 2 if DropoutUnit(unit) is DropoutUnit.CHANNEL else 1
+        lead = 2 if unit is DropoutUnit.CHANNEL else 1
         if input_.dim() < lead:
             raise ValueError(f"serron.dropout: unit {unit.value!r} needs an input of at least {lead} dimensions, got "
                              f"{input_.dim()}")

@@ -544,3 +544,23 @@ def test_autocast_leaves_them_alone(serron):
     with torch.autocast("cuda"):
         assert torch.equal(serron.layer_norm(x, w, b), want)
         assert serron.dropout(x.float(), seed=1).dtype == torch.float32
+
+
+def test_example_learns(serron):
+    """The operators together, as a network uses them: the example's loss falls, every parameter gets a gradient, and
+    evaluation drops nothing."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "residual_denoiser.py")
+    spec = importlib.util.spec_from_file_location("residual_denoiser", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    model, losses = example.train(60)
+    assert losses[-1] < 0.5 * losses[0] and all(math.isfinite(v) for v in losses)
+    model.eval()
+    noisy, _ = example.batch(2, 32, torch.Generator("cuda").manual_seed(3))
+    with torch.no_grad():
+        assert torch.equal(model(noisy), model(noisy))
+    for p in model.parameters():
+        assert p.grad is not None and bool(p.grad.isfinite().all())

@@ -145,6 +145,8 @@ def test_dropout_units():
         serron.dropout(_Cuda(torch.rand(4)), seed=1, unit=serron.DropoutUnit.CHANNEL)
     with pytest.raises(ValueError, match="unit 'sample' needs an input of at least 1 dimensions, got 0"):
         serron.dropout(_Cuda(torch.tensor(1.0)), seed=1, unit=serron.DropoutUnit.SAMPLE)
+    with pytest.raises(ValueError, match="'pixel' is not a valid DropoutUnit"):
+        serron.dropout(_Cuda(torch.rand(4, 4)), seed=1, unit="pixel")
 
 
 def test_modules():
