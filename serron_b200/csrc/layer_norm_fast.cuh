@@ -165,6 +165,18 @@ __device__ __forceinline__ Floats<V> got(const float* plane, int lane) {
     return Pack<float, V>::load(plane + lane * V).floats();
 }
 
+// Brings a thread's strides of the next tile from DRAM to the L2 while the present one is computed on.  The lanes of a warp share the
+// lines: kPer lanes' vectors lie in one, and each of those asks for another stride or tensor, at its own place in the row.
+template <typename T, int V, int NV>
+__device__ __forceinline__ void fetch_ahead(const T* const (&from)[3], int tensors, unsigned step, int count) {
+    constexpr int kBytes = V * static_cast<int>(sizeof(T)), kPer = kBytes >= 4 ? 128 / kBytes : 32;
+    for (int i = static_cast<int>(threadIdx.x & 31) % kPer; i < tensors * NV; i += kPer) {
+        const int m = i / NV, k = i % NV;
+        const T* p = (m == 0 ? from[0] : m == 1 ? from[1] : from[2]) + k * step;
+        if (k < count) asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+    }
+}
+
 // Sums M numbers for each of a lane's V rows over the groups of a block, then over the blocks of a cluster.  `shared`:
 // [2 phases][M][groups][lanes][V], then for the cluster [2 phases][M][lanes][V]; `phase` alternates from call to call, so that a
 // call's reads and the next but one's writes have a barrier between them.
@@ -237,11 +249,16 @@ __global__ void __maxnreg__(JOIN ? 128 : 96) norm_columns_kernel(const __grid_co
     }
 
     int phase = 0;
+    long long next = 0;  // where the thread's part of the next tile begins
+    bool next_live = false;
+    const auto look = [&](long long t) {
+        next_live = column_place<V>(a.shape, t * lanes + lane, next);
+        next += static_cast<long long>(group) * a.shape.inner;
+    };
+    look(blockIdx.x);
     for (long long t = blockIdx.x; t < a.tiles; t += gridDim.x) {
-        const long long q = t * lanes + lane;
-        long long offset;
-        const bool live = column_place<V>(a.shape, q, offset);
-        const long long first = offset + static_cast<long long>(group) * a.shape.inner;
+        const long long q = t * lanes + lane, first = next;
+        const bool live = next_live;
         P h[NV];
         F sum[1], squares[1];
         sum[0].fill(0.0f);
@@ -254,6 +271,12 @@ __global__ void __maxnreg__(JOIN ? 128 : 96) norm_columns_kernel(const __grid_co
                     h[k] = P::load(a.x + first + k * step);
                     if (JOIN) res[k] = P::load(a.residual + first + k * step);
                 }
+            }
+            if (t + gridDim.x < a.tiles) {
+                look(t + gridDim.x);
+                if (next_live)
+                    fetch_ahead<T, V, NV>({a.x + next, JOIN ? a.residual + next : nullptr, nullptr}, JOIN ? 2 : 1, step,
+                                          count);
             }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
@@ -351,12 +374,20 @@ __global__ void __maxnreg__(128) norm_columns_bwd_kernel(const __grid_constant__
         dw[k] = db[k] = splat<E>(0.0f);
     }
 
+    // the join of 16-bit vectors has no registers left for the next tile's place: 361 us at (64,32,256,256) bfloat16, 372 with it
+    constexpr bool kFetch = !(JOIN && sizeof(T) == 2 && V > 1);
     int phase = 0;
+    long long next = 0;  // where the thread's part of the next tile begins
+    bool next_live = false;
+    const auto look = [&](long long t) {
+        next_live = column_place<V>(a.shape, t * lanes + lane, next);
+        next += static_cast<long long>(group) * a.shape.inner;
+    };
+    if (kFetch) look(blockIdx.x);
     for (long long t = blockIdx.x; t < a.tiles; t += gridDim.x) {
-        const long long q = t * lanes + lane;
-        long long offset;
-        const bool live = column_place<V>(a.shape, q, offset);
-        const long long first = offset + static_cast<long long>(group) * a.shape.inner;
+        if (!kFetch) look(t);
+        const long long q = t * lanes + lane, first = next;
+        const bool live = next_live;
         P gy[NV], x[NV], extra[JOIN ? NV : 1];
         F mean, rstd, s[2];
         s[0].fill(0.0f);
@@ -386,6 +417,12 @@ __global__ void __maxnreg__(128) norm_columns_bwd_kernel(const __grid_constant__
 #pragma unroll
                 for (int k = 0; k < NV; ++k)
                     if (FULL || k < count) extra[k] = P::load(a.add + first + k * step);
+            }
+            if (kFetch && t + gridDim.x < a.tiles) {
+                look(t + gridDim.x);
+                if (next_live)
+                    fetch_ahead<T, V, NV>({a.gy + next, a.x + next, JOIN ? a.add + next : nullptr},
+                                          JOIN && a.add != nullptr ? 3 : 2, step, count);
             }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
@@ -782,6 +819,17 @@ __global__ void __maxnreg__(128) norm_rows_bwd_kernel(const __grid_constant__ No
                     if (JOIN && a.add != nullptr)
                         extra[r][k] = load_part<T, V, SHIFTED>(a.add, e, whole, inside, lo, hi);
                 }
+            }
+        }
+        if (t + gridDim.x < a.tiles) {
+            // the next tile from DRAM to the L2: eight lanes' vectors lie in a line, each asks for another one's
+            constexpr int kPer = V * sizeof(T) == 16 ? 8 : 32;
+            const long long ahead = place.row(t + gridDim.x, R);
+            for (int i = threadIdx.x % kPer; i < 2 * R * NV; i += kPer) {
+                const int r = i / NV % R, j = place.first + i % NV * place.all;
+                const long long row = ahead + r * place.kStep;
+                const T* p = (i < R * NV ? a.gy : a.x) + place.at(ahead) + r * row_step + i % NV * place.all * V;
+                if (row < a.shape.rows && j < place.vectors) asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
             }
         }
         E p1[R], p2[R];

@@ -204,9 +204,16 @@ void param_final(const typename Storage<T>::acc* sums, int64_t blocks, int len, 
     int shares = 1;
     while (shares < 32 && blocks >= 16 * shares) shares *= 2;
     const int columns = std::max(32, 128 / shares);
-    norm_param_final_kernel<T><<<static_cast<unsigned>(ceil_div64(2ll * len, columns)), dim3(columns, shares), 0,
-                                 stream>>>(sums, static_cast<int>(blocks), len, dw, db, f32);
-    SB_CUDA(cudaGetLastError());
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(ceil_div64(2ll * len, columns)));
+    config.blockDim = dim3(columns, shares);
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    SB_CUDA(cudaLaunchKernelEx(&config, norm_param_final_kernel<T>, sums, static_cast<int>(blocks), len, dw, db, f32));
 }
 
 template <typename T>
