@@ -78,6 +78,16 @@ void launch_dropout(const char* name, const void* x_, const void* residual_, voi
             SB_CUDA(cudaGetLastError());
             return;
         }
+        if (wide && span >= V && (span < kLongSpan || (span % V != 0 && span < (int64_t(1) << 30)))) {
+            const unsigned blocks = grid_of(name, ceil_div64(n, 256 * U * V));
+            auto kernel = rule.seed_device ? (residual ? dropout_spans_kernel<T, V, U, true, true>
+                                                       : dropout_spans_kernel<T, V, U, false, true>)
+                                           : (residual ? dropout_spans_kernel<T, V, U, true, false>
+                                                       : dropout_spans_kernel<T, V, U, false, false>);
+            kernel<<<blocks, 256, 0, stream>>>(x, residual, y, n, static_cast<int>(span), rule);
+            SB_CUDA(cudaGetLastError());
+            return;
+        }
         if (span >= 256 && n % span == 0) {
             const int64_t width = wide && span % V == 0 ? V : 1;
             const int64_t pieces = ceil_div64(span, 256 * U * width);

@@ -284,7 +284,8 @@ def test_dropout_elements(serron, n, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("shape", [(3, 5), (2, 3, 1), (4, 6, 2), (5, 3, 3), (3, 7, 5, 1), (2, 9, 4, 8), (6, 5, 7, 9), (2, 16, 32, 33),
-                                   (1, 3, 100, 100)])
+                                   (1, 3, 100, 100), (40, 33, 7, 7), (8, 64, 14, 14), (3, 1001, 13), (5, 1700, 8), (2, 3, 8191),
+                                   (2, 3, 8192), (1, 2, 70001)])
 def test_dropout_units(serron, shape, dtype):
     x, r = _rand(shape, dtype, 1), _rand(shape, dtype, 2)
     for unit, lead in ((serron.DropoutUnit.CHANNEL, 2), (serron.DropoutUnit.SAMPLE, 1)):
