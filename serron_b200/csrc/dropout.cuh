@@ -9,7 +9,12 @@ namespace serron {
 
 // Decisions by element, p < 1.  A thread takes U vectors of V consecutive elements, 256 vectors apart, all loads issued
 // before the first is used; a block of the generator serves four elements.  A block's elements start at a multiple of
-// their number, a power of two, so the upper word of the generator's counter is the same for all of them.
+// their number, a power of two, so the upper word of the generator's counter is the same for all of them, and with it
+// half of the first two rounds.  The round keys are operands in constant memory where the seed is the host's.
+//
+// 16-bit elements are bound by the generator: five 32 x 32 -> 64 bit products an element, 17 instructions in all (26 with keys
+// made in the kernel and elements unpacked one at a time).  (64,32,256,256) bfloat16: 104 us (5.2 TB/s, 79 % of the copy
+// rate), with a residual 117 (at the copy rate, part of it from the L2); float32 runs at 90 to 100 % of it.
 template <typename T, int V, int U, bool RESIDUAL, bool DEVICE_SEED>
 __global__ void __launch_bounds__(256)
     dropout_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __restrict__ y, long long n,
@@ -85,15 +90,15 @@ __global__ void __launch_bounds__(256)
     y[e] = S::store(v);
 }
 
-// Decisions by channel or sample, `span` elements each, V <= span < 2^30: small maps, of which a block holds many, and any that begin
-// off a vector's boundary.  Vectors as above; a vector's first unit is found from where the block begins, and a vector may hold
-// the end of one unit and the beginning of the next.  The input is read only where something is kept.  (64,512,14,14) float16: 10.3 us;
-// a block to a unit, or a thread to an element, took 40.
+// Decisions by channel or sample, `span` elements each, V <= span < 2^30: small maps, of which a block holds many, and any
+// that begin off a vector's boundary.  Vectors as above; a vector's first unit is found from where the block begins, and
+// a vector may hold the end of one unit and the beginning of the next.  The input is read only where something is kept.
+// (64,512,14,14) float16: 10.3 us; a decision for every element by itself took 40.
 constexpr int kLongSpan = 8192;
 template <typename T, int V, int U, bool RESIDUAL, bool DEVICE_SEED>
 __global__ void __launch_bounds__(256)
-    dropout_spans_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __restrict__ y, long long n, int span,
-                         const __grid_constant__ DropRule rule) {
+    dropout_spans_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __restrict__ y, long long n,
+                         int span, const __grid_constant__ DropRule rule) {
     using P = Pack<T, V>;
     using F = Floats<V>;
     static_assert(256 * U * V <= kLongSpan);
@@ -155,7 +160,8 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
             for (int k = 0; k < V; ++k) {  // the last, incomplete vector
                 if (e + k < left) {
-                    float v = (k < ends[u] ? kept[u] : after[u]) ? scaled(Storage<T>::load(xs[e + k]), rule.scale32) : 0.0f;
+                    const bool keep = k < ends[u] ? kept[u] : after[u];
+                    float v = keep ? scaled(Storage<T>::load(xs[e + k]), rule.scale32) : 0.0f;
                     if (RESIDUAL) v += Storage<T>::load(rs[e + k]);
                     ys[e + k] = Storage<T>::store(v);
                 }
@@ -164,8 +170,9 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// Decisions by channel or sample of kLongSpan elements or more, in whole vectors: a block takes a piece of one unit, decides once and
-// reads the input only where it is kept.  Grid: pieces of a unit, units.
+// Decisions by channel or sample of kLongSpan elements or more, in whole vectors: a block takes a piece of one unit, decides
+// once and reads the input only where it is kept (70 us at (64,32,256,256) bfloat16 with p = 1/4: 7/8 of two passes at the
+// copy rate).  Grid: pieces of a unit, units.
 template <typename T, int V, int U>
 __global__ void __launch_bounds__(256)
     dropout_units_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __restrict__ y, long long span,

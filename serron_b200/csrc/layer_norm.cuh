@@ -224,7 +224,8 @@ __global__ void __launch_bounds__(kNormThreads)
     part[(block * 2 + 1) * s.len + l] = db;
 }
 
-// inner == 1 and few rows: a thread owns an element of the row, and what it adds up is the gradient.
+// inner == 1 and few rows: a thread owns an element of the row, and what it adds up is the gradient.  Partial sums of so
+// few rows would be as large as the tensors: 16 rows of 65536 bfloat16 take 14 us with this, 31 with them.
 template <typename T>
 __global__ void __launch_bounds__(128)
     norm_param_direct_kernel(const T* __restrict__ gy, const T* __restrict__ x,
@@ -275,8 +276,8 @@ __global__ void __launch_bounds__(kNormThreads)
     }
 }
 
-// A block sums blockDim.x of the 2 * len columns (dw, then db), each in blockDim.y shares of the partial sums.  It is launched
-// while the kernel that writes them still runs, and waits for its end: a backward pass takes 0.7 to 1.2 us less.
+// A block sums blockDim.x of the 2 * len columns (dw, then db), each in blockDim.y shares of the partial sums.  It is
+// launched while the kernel that writes them still runs, and waits for its end: a backward pass takes 0.7 to 1.2 us less.
 constexpr int kParamThreads = 1024;
 template <typename T>
 __global__ void __launch_bounds__(kParamThreads)

@@ -1,5 +1,5 @@
-// Register kernels of layer norm and the join for __half, in a translation unit of their own so that they compile in
-// parallel.
+// Register kernels of layer norm and the join for __half, in a translation unit of their own
+// so that they compile in parallel.
 #include "layer_norm_launch.cuh"
 
 namespace serron {

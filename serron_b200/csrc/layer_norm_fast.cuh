@@ -9,12 +9,16 @@
 //   columns  (inner  > 1): threadIdx.x counts vectors of V neighbouring rows (neighbours in memory), threadIdx.y the
 //            strides of the normalised dimension
 //
-// The forward pass adds up a row twice over its registers, for the mean and for the squares about that mean, so that a level far
-// above the spread costs nothing; the backward pass adds up two numbers once.
+// The forward pass adds up a row twice over its registers, for the mean and for the squares about that mean, so that a
+// level far above the spread costs nothing; the backward pass adds up two numbers once.  Statistics, sums and
+// products are float32; what is stored in 16 bits is rounded once.
 //
-// These kernels would be bound by instructions, not by memory, if written one float at a time (31 instructions an element
-// of a row, 48 of a column, where 16-bit elements leave about 20 at the memory's rate): elements are unpacked
-// once and computed on in pairs (layer_vec.cuh), and divisions are one multiplication and one correction.
+// What bounds them: instructions.  The memory's rate leaves 16-bit elements about 20 instructions each at full issue.  One
+// float at a time the forward pass took 31 an element of a row and 48 of a column; computed on in pairs (layer_vec.cuh),
+// with divisions as one multiplication and one correction, it takes 23 and 15, the backward pass 25 and 24, and the
+// generator adds 19 to 28 in the join.  Warps issue in 52 to 68 % of the cycles (16 to 28 of them are resident).
+//   (64,32,256,256) bfloat16, columns: norm 99 us forward (5.4 TB/s, 83 % of the copy rate of 6.55), 165 backward (74 %);
+//   join 254 (65 %) and 361 (57 %).  (8192,1024) bfloat16, rows: 10.9 and 21.3 us; join 19.9 and 31.6.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -25,7 +29,6 @@
 namespace serron {
 
 namespace cg = cooperative_groups;
-
 
 template <typename T>
 struct NormArgs {
@@ -66,8 +69,8 @@ __device__ __forceinline__ float root_inverse(float v) {
 }
 
 // What the kernels are compiled for: the norm alone, or the join with the generator's keys as operands in constant memory
-// (a seed from the host) or in shared memory (any seed).  The backward pass of columns always has them in shared memory: beside its
-// other registers, operands made it slower (378 us against 360 at (64,32,256,256) bfloat16).
+// (a seed from the host) or in shared memory (any seed).  The backward pass of columns always has them in shared
+// memory: beside its other registers, operands made it slower (378 us against 361 at (64,32,256,256) bfloat16).
 enum Join : int { kNoJoin = 0, kHostSeed = 1, kAnySeed = 2 };
 
 template <int JOIN>
@@ -99,7 +102,8 @@ __device__ __forceinline__ Floats<V> drop(const Floats<V>& v, long long e, const
     return dropped<V>(v, words, rule.threshold, rule.scale32);
 }
 
-// residual + dropout(x), rounded to T
+// residual + dropout(x), rounded to T: it is an output, and the norm (and its backward pass, which reads it back) is of
+// that output.
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> joined(const Pack<T, V>& x, const Pack<T, V>& residual, long long e,
                                              const DropRule& rule, const PhiloxKeys& keys) {
@@ -165,8 +169,11 @@ __device__ __forceinline__ Floats<V> got(const float* plane, int lane) {
     return Pack<float, V>::load(plane + lane * V).floats();
 }
 
-// Brings a thread's strides of the next tile from DRAM to the L2 while the present one is computed on.  The lanes of a warp share the
-// lines: kPer lanes' vectors lie in one, and each of those asks for another stride or tensor, at its own place in the row.
+// Brings a thread's strides of the next tile from DRAM to the L2 while the present one is computed on.  The lanes of a warp
+// share the lines: kPer lanes' vectors lie in one, and each of those asks for another stride or tensor, at its own
+// place in the row.  (16,64,128,128) float32: 25 us forward against 30, 51 backward against 58.  Copies of whole tiles into
+// shared memory instead, ahead of their use, cost more instructions than they saved waiting (16-bit: 113 us against 105
+// forward, 176 against 165 backward).
 template <typename T, int V, int NV>
 __device__ __forceinline__ void fetch_ahead(const T* const (&from)[3], int tensors, unsigned step, int count) {
     constexpr int kBytes = V * static_cast<int>(sizeof(T)), kPer = kBytes >= 4 ? 128 / kBytes : 32;
@@ -178,8 +185,8 @@ __device__ __forceinline__ void fetch_ahead(const T* const (&from)[3], int tenso
 }
 
 // Sums M numbers for each of a lane's V rows over the groups of a block, then over the blocks of a cluster.  `shared`:
-// [2 phases][M][groups][lanes][V], then for the cluster [2 phases][M][lanes][V]; `phase` alternates from call to call, so that a
-// call's reads and the next but one's writes have a barrier between them.
+// [2 phases][M][groups][lanes][V], then for the cluster [2 phases][M][lanes][V]; `phase` alternates from call to call, so
+// that a call's reads and the next but one's writes have a barrier between them.
 template <int V, int M>
 __device__ __forceinline__ void column_totals(Floats<V> (&v)[M], float* shared, int& phase) {
     const int lanes = blockDim.x, groups = blockDim.y, lane = threadIdx.x, clusters = gridDim.y, plane = lanes * V;
@@ -223,6 +230,8 @@ __device__ __forceinline__ void column_totals(Floats<V> (&v)[M], float* shared, 
 }
 
 // FULL: every thread has all of its NV strides (len is their number times the groups').
+// Registers: at 96 (five blocks of 128 threads to an SM) the norm at (64,32,256,256) bfloat16 took 102 us, at 128 110, at 80 106, at
+// 64 (spilling) 128; the join 278 at 128 and 318, 331, 402 at 96, 80, 64.
 template <typename T, int V, int NV, int JOIN, bool FULL>
 __global__ void __maxnreg__(JOIN ? 128 : 96) norm_columns_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
@@ -346,7 +355,8 @@ __global__ void __maxnreg__(JOIN ? 128 : 96) norm_columns_kernel(const __grid_co
 }
 
 // A thread adds up its channels' gradients over the tiles that its block (cluster) walks over.  `part` gets
-// [gridDim.x][2][len] sums.
+// [gridDim.x][2][len] sums.  Four blocks of 128 threads to an SM hide more than what fewer registers spill: 167 us at 128
+// registers, 174, 227, 292 at 112, 96, 80, and 246 with 144 (three blocks).
 template <typename T, int V, int NV, int JOIN, bool FULL>
 __global__ void __maxnreg__(128) norm_columns_bwd_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
@@ -374,7 +384,8 @@ __global__ void __maxnreg__(128) norm_columns_bwd_kernel(const __grid_constant__
         dw[k] = db[k] = splat<E>(0.0f);
     }
 
-    // the join of 16-bit vectors has no registers left for the next tile's place: 361 us at (64,32,256,256) bfloat16, 372 with it
+    // the join of 16-bit vectors has no registers left for the next tile's place: 361 us at (64,32,256,256) bfloat16, 372
+    // with it
     constexpr bool kFetch = !(JOIN && sizeof(T) == 2 && V > 1);
     int phase = 0;
     long long next = 0;  // where the thread's part of the next tile begins
@@ -618,7 +629,8 @@ struct RowPlace {
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < V; ++i) f[i] = from + i >= 0 && from + i < len ? load_param<T>(p, from + i, f32) : fill;
+                for (int i = 0; i < V; ++i)
+                    f[i] = from + i >= 0 && from + i < len ? load_param<T>(p, from + i, f32) : fill;
             }
             float cut[V];
 #pragma unroll
@@ -648,8 +660,11 @@ __device__ __forceinline__ Pack<T, V> load_part(const T* p, long long e, bool wh
     return Pack<T, V>::of(v);
 }
 
+// Registers: 64 for whole vectors (11.1 us at (8192,1024) bfloat16; at 80, 96, 128 12.2, 12.1, 12.4), 80 in the join, which at 64
+// is slower for short rows (200,000 of 64: 33 us against 30); 32 more where vectors are shifted, which spilled.
 template <typename T, int V, int NV, int R, int JOIN, bool SHIFTED>
-__global__ void __maxnreg__((JOIN ? 80 : 64) + (SHIFTED ? 32 : 0)) norm_rows_kernel(const __grid_constant__ NormArgs<T> a) {
+__global__ void __maxnreg__((JOIN ? 80 : 64) + (SHIFTED ? 32 : 0))
+    norm_rows_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
     using F = Floats<V>;
     using E = typename F::E;
@@ -675,7 +690,8 @@ __global__ void __maxnreg__((JOIN ? 80 : 64) + (SHIFTED ? 32 : 0)) norm_rows_ker
         P h[R][NV];
         float sum[R], squares[R], mean[R], rstd[R];
         const long long row0 = place.row(t, R), base = place.at(row0);
-        const int rows = static_cast<int>(min((a.shape.rows - row0 + place.kStep - 1) / place.kStep, static_cast<long long>(R)));
+        const int rows =
+            static_cast<int>(min((a.shape.rows - row0 + place.kStep - 1) / place.kStep, static_cast<long long>(R)));
         {
             P res[JOIN ? R : 1][NV];
 #pragma unroll
@@ -771,7 +787,8 @@ __global__ void __maxnreg__((JOIN ? 80 : 64) + (SHIFTED ? 32 : 0)) norm_rows_ker
     if (gridDim.y > 1) cg::this_cluster().sync();  // no block leaves while another reads it
 }
 
-// `part` gets [gridDim.x][2][len] sums of the parameters' gradients, one pair per block (cluster).
+// `part` gets [gridDim.x][2][len] sums of the parameters' gradients, one pair per block (cluster).  Registers: 22 us at
+// (8192,1024) bfloat16 with 128; 25, 27, 34 with 96, 80, 64.
 template <typename T, int V, int NV, int R, int JOIN, bool SHIFTED>
 __global__ void __maxnreg__(128) norm_rows_bwd_kernel(const __grid_constant__ NormArgs<T> a) {
     using P = Pack<T, V>;
@@ -801,7 +818,8 @@ __global__ void __maxnreg__(128) norm_rows_bwd_kernel(const __grid_constant__ No
         P gy[R][NV], x[R][NV], extra[JOIN ? R : 1][NV];
         float mean[R], rstd[R], s[2 * R];
         const long long row0 = place.row(t, R), base = place.at(row0);
-        const int rows = static_cast<int>(min((a.shape.rows - row0 + place.kStep - 1) / place.kStep, static_cast<long long>(R)));
+        const int rows =
+            static_cast<int>(min((a.shape.rows - row0 + place.kStep - 1) / place.kStep, static_cast<long long>(R)));
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const bool live = r < rows;

@@ -81,7 +81,8 @@ cudaError_t norm_launch(const NormPlan& p, bool backward, int join, const NormAr
     if (p.V == v && p.NV == nv && p.R == r && p.shifted == off) \
         return launch_rows<T, v, nv, r, off>(p, backward, join, args, stream);
 #define SERRON_COLUMNS_CASE(v, nv, whole) \
-    if (p.V == v && p.NV == nv && p.full == whole) return launch_columns<T, v, nv, whole>(p, backward, join, args, stream);
+    if (p.V == v && p.NV == nv && p.full == whole) \
+        return launch_columns<T, v, nv, whole>(p, backward, join, args, stream);
     if (p.rows) {
         SERRON_ROWS_CASE(W, 1, 4, false)
         SERRON_ROWS_CASE(W, 1, 1, false)

@@ -210,7 +210,7 @@ __device__ __forceinline__ Floats<V> load_params(const void* p, int i, bool f32)
     }
 }
 
-// The words of decisions e .. e + V - 1, where e is a multiple of min(V, 4) and below 2^34.
+// The words of decisions e .. e + V - 1 (below 2^34), where e is a multiple of V.
 template <int V>
 __device__ __forceinline__ void drop_words(long long e, uint64_t sequence, const PhiloxKeys& keys, uint32_t (&out)[V]) {
     if constexpr (V >= 4) {
@@ -223,13 +223,8 @@ __device__ __forceinline__ void drop_words(long long e, uint64_t sequence, const
             out[k + 3] = w.w;
         }
     } else {
-        const uint4 w = philox(static_cast<uint32_t>(e >> 2), 0u, sequence, keys);
-        if constexpr (V == 2) {
-            out[0] = e & 2 ? w.z : w.x;
-            out[1] = e & 2 ? w.w : w.y;
-        } else {
-            out[0] = word_of(w, e & 3);
-        }
+        static_assert(V == 1);
+        out[0] = word_of(philox(static_cast<uint32_t>(e >> 2), 0u, sequence, keys), e & 3);
     }
 }
 
