@@ -641,23 +641,20 @@ struct RowPlace {
     }
 };
 
-// The V elements from e on; of an incomplete vector those before lo and from hi on, another row's, read as zero.
-// `inside`: the whole vector lies in the tensor, which has no more than the last one's end beyond it.
-template <typename T, int V, bool SHIFTED>
-__device__ __forceinline__ Pack<T, V> load_part(const T* p, long long e, bool whole, bool inside, int lo, int hi) {
-    if (!SHIFTED || whole) return Pack<T, V>::load(p + e);
+// An incomplete vector with zeros in the place of other rows' elements, before lo and from hi on.  `inside`: it lies in the tensor
+// and was read as a whole (all but the tensor's last are); else its own elements are read now, one by one.
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> trimmed(const Pack<T, V>& v, const T* p, bool inside, int lo, int hi) {
     float f[V];
-    if (inside) {
-        Pack<T, V>::load(p + e).floats().to(f);
-    } else {
+    v.floats().to(f);
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = i < hi ? Storage<T>::load(p[e + i]) : 0.0f;
+    for (int i = 0; i < V; ++i) {
+        if (!inside) f[i] = i < hi ? Storage<T>::load(p[i]) : 0.0f;
+        f[i] = i >= lo && i < hi ? f[i] : 0.0f;
     }
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = i >= lo && i < hi ? f[i] : 0.0f;
-    Floats<V> v;
-    v.from(f);
-    return Pack<T, V>::of(v);
+    Floats<V> out;
+    out.from(f);
+    return Pack<T, V>::of(out);
 }
 
 // Registers: 64 for whole vectors (11.1 us at (8192,1024) bfloat16; at 80, 96, 128 12.2, 12.1, 12.4), 80 in the join, which at 64
@@ -674,7 +671,7 @@ __global__ void __maxnreg__((JOIN ? 80 : 64) + (SHIFTED ? 32 : 0))
     __shared__ PhiloxKeys own_keys;
     const RowPlace<V, SHIFTED> place(a.shape);
     const float n = static_cast<float>(place.len), inverse = 1.0f / n;
-    const long long row_step = static_cast<long long>(place.len) * place.kStep;
+    const long long row_step = static_cast<long long>(place.len) * place.kStep, numel = a.shape.rows * place.len;
     const PhiloxKeys& keys = join_keys<JOIN>(a.rule, own_keys);
     F w[NV], b[NV];
     if (kKeepParams) {
@@ -701,10 +698,26 @@ __global__ void __maxnreg__((JOIN ? 80 : 64) + (SHIFTED ? 32 : 0))
                     const int j = place.first + k * place.all;
                     if (r < rows && j < place.vectors) {
                         const long long e = base + r * row_step + k * place.all * V;
-                        const bool whole = place.whole(j), inside = e + V <= a.shape.rows * place.len;
-                        const int lo = place.lo(j), hi = place.hi(j);
-                        h[r][k] = load_part<T, V, SHIFTED>(a.x, e, whole, inside, lo, hi);
-                        if (JOIN) res[r][k] = load_part<T, V, SHIFTED>(a.residual, e, whole, inside, lo, hi);
+                        if (!SHIFTED || e + V <= numel) {
+                            h[r][k] = P::load(a.x + e);
+                            if (JOIN) res[r][k] = P::load(a.residual + e);
+                        }
+                    }
+                }
+            }
+            if (SHIFTED) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+#pragma unroll
+                    for (int k = 0; k < NV; ++k) {
+                        const int j = place.first + k * place.all;
+                        if (r < rows && j < place.vectors && !place.whole(j)) {
+                            const long long e = base + r * row_step + k * place.all * V;
+                            const bool inside = e + V <= numel;
+                            h[r][k] = trimmed<T, V>(h[r][k], a.x + e, inside, place.lo(j), place.hi(j));
+                            if (JOIN)
+                                res[r][k] = trimmed<T, V>(res[r][k], a.residual + e, inside, place.lo(j), place.hi(j));
+                        }
                     }
                 }
             }
@@ -801,7 +814,7 @@ __global__ void __maxnreg__(128) norm_rows_bwd_kernel(const __grid_constant__ No
     __shared__ PhiloxKeys own_keys;
     const RowPlace<V, SHIFTED> place(a.shape);
     const float inverse = 1.0f / static_cast<float>(place.len);
-    const long long row_step = static_cast<long long>(place.len) * place.kStep;
+    const long long row_step = static_cast<long long>(place.len) * place.kStep, numel = a.shape.rows * place.len;
     const bool stores = a.dx != nullptr || (JOIN && a.dropped != nullptr);
     const PhiloxKeys& keys = join_keys<JOIN>(a.rule, own_keys);
 
@@ -828,14 +841,29 @@ __global__ void __maxnreg__(128) norm_rows_bwd_kernel(const __grid_constant__ No
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 const int j = place.first + k * place.all;
-                if (live && j < place.vectors) {
-                    const long long e = base + r * row_step + k * place.all * V;
-                    const bool whole = place.whole(j), inside = e + V <= a.shape.rows * place.len;
-                    const int lo = place.lo(j), hi = place.hi(j);
-                    gy[r][k] = load_part<T, V, SHIFTED>(a.gy, e, whole, inside, lo, hi);
-                    x[r][k] = load_part<T, V, SHIFTED>(a.x, e, whole, inside, lo, hi);
-                    if (JOIN && a.add != nullptr)
-                        extra[r][k] = load_part<T, V, SHIFTED>(a.add, e, whole, inside, lo, hi);
+                const long long e = base + r * row_step + k * place.all * V;
+                if (live && j < place.vectors && (!SHIFTED || e + V <= numel)) {
+                    gy[r][k] = P::load(a.gy + e);
+                    x[r][k] = P::load(a.x + e);
+                    if (JOIN && a.add != nullptr) extra[r][k] = P::load(a.add + e);
+                }
+            }
+        }
+        if (SHIFTED) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    const int j = place.first + k * place.all;
+                    if (r < rows && j < place.vectors && !place.whole(j)) {
+                        const long long e = base + r * row_step + k * place.all * V;
+                        const bool inside = e + V <= numel;
+                        const int lo = place.lo(j), hi = place.hi(j);
+                        gy[r][k] = trimmed<T, V>(gy[r][k], a.gy + e, inside, lo, hi);
+                        x[r][k] = trimmed<T, V>(x[r][k], a.x + e, inside, lo, hi);
+                        if (JOIN && a.add != nullptr)
+                            extra[r][k] = trimmed<T, V>(extra[r][k], a.add + e, inside, lo, hi);
+                    }
                 }
             }
         }
