@@ -220,7 +220,7 @@ SERRON_API int serron_derived_forward(int32_t mode, const void* input, const int
  *   - `weight` and `bias` (len elements each; either may be NULL) are float32 or of the input's dtype, as
  *     `param_dtype` says for both.
  *   - `mean` and `rstd` (outer * inner elements, row (o, i) at o * inner + i; float32, or float64 for
- *     float64 inputs) are what the backward reads; both may be NULL where none follows.
+ *     float64 inputs) are what the backward reads; both are NULL where none follows (one alone is refused).
  *   - the backward gives grad_input, grad_weight and grad_bias (the last two of `param_dtype`), each
  *     skipped where NULL, in sums whose order depends on the sizes alone.
  *   - workspace: serron_layer_norm_workspace_bytes bytes, 256-byte aligned; -1 (with a message) for

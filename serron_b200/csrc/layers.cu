@@ -352,6 +352,11 @@ void check_workspace(const char* name, const void* workspace, int64_t have, int6
         throw Failure{SERRON_ERR_WORKSPACE, concat(name, ": workspace of ", have, " bytes, ", need, " needed")};
 }
 
+// The kernels write both statistics where they write the mean.
+void check_stats(const char* name, const void* mean, const void* rstd) {
+    SB_CHECK((mean == nullptr) == (rstd == nullptr), name, ": mean and rstd are given both or not at all");
+}
+
 // No rows: nothing to normalise, and gradients of the parameters that are sums of nothing.
 void zero_params(int len, int param_dtype, void* dw, void* db, cudaStream_t stream) {
     if (dw) SB_CUDA(cudaMemsetAsync(dw, 0, len * elem_size(param_dtype), stream));
@@ -408,6 +413,7 @@ int serron_layer_norm(const void* input, int64_t outer, int64_t len, int64_t inn
         check_norm(name, dtype, param_dtype, weight, bias);
         SB_CHECK(eps >= 0.0 && std::isfinite(eps), name, ": eps must be finite and not negative, got ", eps);
         const Norm n = norm_of(name, outer, len, inner);
+        check_stats(name, mean, rstd);
         if (n.numel() == 0) return;
         SB_CHECK(input && output, name, ": tensors must not be null");
         check_workspace(name, workspace, workspace_bytes, workspace_bytes_of(n, dtype, false));
@@ -459,6 +465,7 @@ int serron_dropout_add_layer_norm(const void* input, const void* residual, int64
         SB_CHECK(eps >= 0.0 && std::isfinite(eps), name, ": eps must be finite and not negative, got ", eps);
         const Norm n = norm_of(name, outer, len, inner);
         const DropRule rule = drop_rule(name, p, seed, seed_device, sequence);
+        check_stats(name, mean, rstd);
         if (n.numel() == 0) return;
         SB_CHECK(input && residual && sum && output, name, ": tensors must not be null");
         check_workspace(name, workspace, workspace_bytes, workspace_bytes_of(n, dtype, false));
