@@ -50,10 +50,11 @@ __device__ __forceinline__ A row_sum(A v, A* shared) {
     return s;
 }
 
-// What a thread of the chunk kernels works on.
+// What a thread of the chunk kernels works on: elements first, first + step, ... below `end` of a row.  A row may have
+// 2^31 - 1 elements, and the index that leaves the loop lies up to `step` beyond them.
 struct ChunkPlace {
     long long row, offset;
-    int first, step, end;
+    unsigned first, step, end;
     bool live;
 };
 template <bool ROWS>
@@ -63,8 +64,8 @@ __device__ __forceinline__ ChunkPlace chunk_place(const NormShape& s, int chunk,
     p.live = p.row < s.rows;
     p.offset = p.live ? s.base(p.row) : 0;
     const long long begin = static_cast<long long>(split) * chunk;
-    p.end = p.live ? static_cast<int>(min(begin + chunk, static_cast<long long>(s.len))) : 0;
-    p.first = static_cast<int>(begin) + (ROWS ? threadIdx.x : threadIdx.x >> 5);
+    p.end = p.live ? static_cast<unsigned>(min(begin + chunk, static_cast<long long>(s.len))) : 0u;
+    p.first = static_cast<unsigned>(begin) + (ROWS ? threadIdx.x : threadIdx.x >> 5);
     p.step = ROWS ? kNormThreads : kNormThreads / 32;
     return p;
 }
@@ -80,10 +81,10 @@ __global__ void __launch_bounds__(kNormThreads)
     const ChunkPlace p = chunk_place<ROWS>(s, chunk, split);
     const int count = min(chunk, s.len - split * chunk);
     A sum = A(0);
-    for (int l = p.first; l < p.end; l += p.step) sum += S::load(x[p.offset + static_cast<long long>(l) * s.inner]);
+    for (unsigned l = p.first; l < p.end; l += p.step) sum += S::load(x[p.offset + static_cast<long long>(l) * s.inner]);
     const A mean = row_sum<ROWS>(sum, shared) / A(count);
     A m2 = A(0);
-    for (int l = p.first; l < p.end; l += p.step) {
+    for (unsigned l = p.first; l < p.end; l += p.step) {
         const A d = S::load(x[p.offset + static_cast<long long>(l) * s.inner]) - mean;
         m2 += d * d;
     }
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(kNormThreads)
     const ChunkPlace p = chunk_place<ROWS>(s, chunk, blockIdx.y);
     if (!p.live) return;
     const A m = mean[p.row], r = rstd[p.row];
-    for (int l = p.first; l < p.end; l += p.step) {
+    for (unsigned l = p.first; l < p.end; l += p.step) {
         const long long e = p.offset + static_cast<long long>(l) * s.inner;
         A v = (S::load(x[e]) - m) * r;
         if (weight) v *= load_param<T>(weight, l, f32);
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(kNormThreads)
     const ChunkPlace p = chunk_place<ROWS>(s, chunk, blockIdx.y);
     const A m = p.live ? mean[p.row] : A(0), r = p.live ? rstd[p.row] : A(0);
     A s1 = A(0), s2 = A(0);
-    for (int l = p.first; l < p.end; l += p.step) {
+    for (unsigned l = p.first; l < p.end; l += p.step) {
         const long long e = p.offset + static_cast<long long>(l) * s.inner;
         A g = S::load(gy[e]);
         if (weight) g *= load_param<T>(weight, l, f32);
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(kNormThreads)
     s1 /= A(s.len);
     s2 /= A(s.len);
     const A m = mean[p.row], r = rstd[p.row];
-    for (int l = p.first; l < p.end; l += p.step) {
+    for (unsigned l = p.first; l < p.end; l += p.step) {
         const long long e = p.offset + static_cast<long long>(l) * s.inner;
         A g = S::load(gy[e]);
         if (weight) g *= load_param<T>(weight, l, f32);

@@ -140,7 +140,8 @@ Norm norm_of(const char* name, int64_t outer, int64_t len, int64_t inner) {
     SB_CHECK(len >= 1, name, ": the normalised dimension must not be empty");
     SB_CHECK(len < (int64_t(1) << 31) && inner < (int64_t(1) << 31), name,
              ": the normalised dimension and the elements behind it must be below 2^31");
-    SB_CHECK(outer == 0 || inner == 0 || outer <= std::numeric_limits<int64_t>::max() / 16 / len / inner, name,
+    // no workspace takes more than 32 bytes an element, and 64 leave room for its alignment
+    SB_CHECK(outer == 0 || inner == 0 || outer <= std::numeric_limits<int64_t>::max() / 64 / len / inner, name,
              ": too many elements");
     Norm n;
     n.shape.rows = outer * inner;
@@ -335,7 +336,7 @@ void norm_backward(const char* name, const Norm& n, const void* gy_, const void*
     }
     if (dw || db) {
         if (rows) {
-            const int tiles = ceil_div(n.shape.len, kNormThreads);
+            const int tiles = static_cast<int>(ceil_div64(n.shape.len, kNormThreads));
             norm_param_rows_kernel<T><<<grid_of(name, n.blocks * tiles), kNormThreads, 0, stream>>>(
                 gy, x, mean, rstd, sums, n.shape, n.rows_per, tiles);
         } else {

@@ -1,0 +1,71 @@
+"""Contracts of the layer operators on the GPU: the top of the index range, tiny spreads, what autograd may hand back,
+captured graphs.  Bounds: layer_oracle.py."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def serron():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    import serron_b200
+
+    return serron_b200
+
+
+def _signs(n, seed):
+    gen = torch.Generator("cuda").manual_seed(seed)
+    out = torch.empty(n, dtype=torch.bfloat16, device="cuda")
+    for part in out.split(1 << 27):
+        part.copy_(torch.randint(0, 2, part.shape, generator=gen, device="cuda", dtype=torch.int8) * 2 - 1)
+    return out
+
+
+def _total(*factors):
+    parts = zip(*(f.split(1 << 27) for f in factors))
+    return sum(float(torch.stack(p).float().prod(0).sum(dtype=torch.float64)) for p in parts)
+
+
+def _near(got, want, bound):
+    """``want`` and ``got`` in pieces; bfloat16 results are rounded once more (2^-8 of values below 4)."""
+    for k, part in enumerate(got.split(1 << 27)):
+        off = (part.float() - want(slice(k << 27, (k << 27) + part.numel()))).abs().amax()
+        assert float(off) <= bound + 2.0**-6, (k, float(off))
+
+
+@pytest.mark.parametrize("inner", [1, 2])
+def test_longest_dimension(serron, inner):
+    """A dimension within a block's stride of 2^31: the index that ends a row's loop does not fit in 31 bits.
+
+    x and grad_output are signs, so |x|, |xhat|, X of the bound are 1 and G is |w| = 1.  The longest chain is the join of
+    65535 chunks, three roundings each, and about 200 within a chunk: K u = 0.012, three times that on y, nine on dx
+    and (for one row) the formula's own product on dw."""
+    length = (1 << 31) - 3
+    chain = (3 * 65535 + 200) * 2.0**-24
+    x = _signs(length * inner, 1)
+    gy = _signs(length * inner, 2)
+    shape = (1, length) if inner == 1 else (1, length, inner)
+    # the columns of inner = 2 are rows of their own
+    columns = [slice(i, None, inner) for i in range(inner)]
+    sums = [(_total(x[c]) / length, _total(gy[c]) / length, _total(gy[c], x[c]) / length) for c in columns]
+    leaves = [x.view(shape).requires_grad_()]
+    if inner == 1:
+        leaves += [torch.ones(length, dtype=torch.bfloat16, device="cuda").requires_grad_(),
+                   torch.zeros(length, dtype=torch.bfloat16, device="cuda").requires_grad_()]
+    y = serron.layer_norm(*leaves, dim=1, eps=0.0)
+    grads = torch.autograd.grad(y, leaves, gy.view(shape))
+    with torch.no_grad():
+        for c, (m, g, gx) in zip(columns, sums):
+            rstd = (1 - m * m) ** -0.5
+            g_xhat = (gx - m * g) * rstd
+            xc, gc = x[c], gy[c]
+            _near(y.view(-1)[c], lambda s: (xc[s].float() - m) * rstd, 3 * chain)
+            _near(grads[0].view(-1)[c], lambda s: rstd * (gc[s].float() - g - (xc[s].float() - m) * rstd * g_xhat), 9 * chain)
+            if inner == 1:
+                _near(grads[1], lambda s: gc[s].float() * (xc[s].float() - m) * rstd, 3 * chain)
+                assert torch.equal(grads[2], gc)

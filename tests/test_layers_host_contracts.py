@@ -23,3 +23,18 @@ def test_one_statistic_alone_is_refused(lib, mean, rstd):
                                                rstd, 256, 1 << 20, 0, None)
         assert rc == _lib.ERR_INVALID
         assert "serron::dropout_add_layer_norm: mean and rstd" in lib.serron_last_error().decode()
+
+
+def test_sizes_at_the_top_of_the_range(lib):
+    """What is accepted has a workspace that 64 bits hold; the rest is refused with a message."""
+    size = lib.serron_layer_norm_workspace_bytes
+    top = (1 << 31) - 1
+    for dtype in range(4):
+        for backward in (0, 1):
+            for outer, length, inner in ((1, top, 1), (1, top, 2), (3, top - 255, 1), (1 << 20, 5, top), (1 << 56, 1, 1)):
+                got = size(outer, length, inner, dtype, backward)
+                assert 0 < got < 1 << 62 and got % 256 == 0
+            for outer, length, inner in ((1 << 59, 1, 1), ((1 << 59) - 1, 1, 1), (1 << 28, top, 1), (1, top, 1 << 27)):
+                if outer * length * inner > ((1 << 63) - 1) // 64:
+                    assert size(outer, length, inner, dtype, backward) == -1
+                    assert "too many elements" in lib.serron_last_error().decode()
