@@ -225,6 +225,8 @@ SERRON_API int serron_derived_forward(int32_t mode, const void* input, const int
  *     skipped where NULL, in sums whose order depends on the sizes alone.
  *   - workspace: serron_layer_norm_workspace_bytes bytes, 256-byte aligned; -1 (with a message) for
  *     arguments no call takes.
+ *   - every tensor starts on a boundary of its elements (a seed in device memory of 8 bytes); other
+ *     addresses are refused, as is a workspace off its 256 bytes.
  *
  * Dropout: y = residual + (kept ? input / (1 - p) : 0), `residual` NULL for none.  Each run of `span`
  * consecutive elements shares one decision (1: every element; H * W: whole channels; C * H * W: whole

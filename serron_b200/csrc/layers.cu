@@ -39,11 +39,20 @@ unsigned grid_of(const char* name, int64_t blocks) {
     return static_cast<unsigned>(blocks);
 }
 
+bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// No kernel can read an element that lies across its own boundary.
+template <typename... P>
+void check_elements(const char* name, size_t size, P... pointers) {
+    SB_CHECK((aligned(pointers, size) && ...), name, ": tensors must start on a boundary of their elements");
+}
+
 // ------------------------------------------------------------------------------------------------
 // dropout
 // ------------------------------------------------------------------------------------------------
 DropRule drop_rule(const char* name, double p, uint64_t seed, const void* seed_device, uint64_t sequence) {
     SB_CHECK(p >= 0.0 && p <= 1.0, name, ": p must be between 0 and 1, got ", p);
+    SB_CHECK(aligned(seed_device, sizeof(uint64_t)), name, ": a seed in device memory must be aligned to 8 bytes");
     DropRule rule;
     rule.keys.set(seed);
     rule.seed_device = static_cast<const uint64_t*>(seed_device);
@@ -55,8 +64,6 @@ DropRule drop_rule(const char* name, double p, uint64_t seed, const void* seed_d
     rule.scale32 = static_cast<float>(rule.scale);
     return rule;
 }
-
-bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 constexpr int kDropVectors = 4;  // per thread
 
@@ -351,10 +358,12 @@ void norm_backward(const char* name, const Norm& n, const void* gy_, const void*
 void check_workspace(const char* name, const void* workspace, int64_t have, int64_t need) {
     if (have < need || (need > 0 && workspace == nullptr))
         throw Failure{SERRON_ERR_WORKSPACE, concat(name, ": workspace of ", have, " bytes, ", need, " needed")};
+    SB_CHECK(need == 0 || aligned(workspace, 256), name, ": the workspace must be aligned to 256 bytes");
 }
 
 // The kernels write both statistics where they write the mean.
-void check_stats(const char* name, const void* mean, const void* rstd) {
+void check_stats(const char* name, int dtype, const void* mean, const void* rstd) {
+    check_elements(name, dtype == kF64 ? 8 : 4, mean, rstd);
     SB_CHECK((mean == nullptr) == (rstd == nullptr), name, ": mean and rstd are given both or not at all");
 }
 
@@ -380,6 +389,9 @@ int layer_norm_backward(const char* name, bool join, const void* grad_output, co
             return zero_params(n.shape.len, param_dtype, grad_weight, grad_bias, stream);
         }
         SB_CHECK(grad_output && input && mean && rstd, name, ": tensors must not be null");
+        check_elements(name, elem_size(dtype), grad_output, grad_sum, input, grad_input, grad_dropped);
+        check_elements(name, elem_size(param_dtype), weight, grad_weight, grad_bias);
+        check_stats(name, dtype, mean, rstd);
         check_workspace(name, workspace, workspace_bytes, workspace_bytes_of(n, dtype, true));
         DeviceScope scope(device);
         with_type(dtype, [&](auto t) {
@@ -414,9 +426,11 @@ int serron_layer_norm(const void* input, int64_t outer, int64_t len, int64_t inn
         check_norm(name, dtype, param_dtype, weight, bias);
         SB_CHECK(eps >= 0.0 && std::isfinite(eps), name, ": eps must be finite and not negative, got ", eps);
         const Norm n = norm_of(name, outer, len, inner);
-        check_stats(name, mean, rstd);
+        check_stats(name, dtype, mean, rstd);
         if (n.numel() == 0) return;
         SB_CHECK(input && output, name, ": tensors must not be null");
+        check_elements(name, elem_size(dtype), input, output);
+        check_elements(name, elem_size(param_dtype), weight, bias);
         check_workspace(name, workspace, workspace_bytes, workspace_bytes_of(n, dtype, false));
         DeviceScope scope(device);
         with_type(dtype, [&](auto t) {
@@ -447,6 +461,7 @@ int serron_dropout(const void* input, const void* residual, int64_t numel, int64
         const DropRule rule = drop_rule(name, p, seed, seed_device, sequence);
         if (numel == 0) return;
         SB_CHECK(input && output, name, ": tensors must not be null");
+        check_elements(name, elem_size(dtype), input, residual, output);
         DeviceScope scope(device);
         with_type(dtype, [&](auto t) {
             launch_dropout<decltype(t)>(name, input, residual, output, numel, span, rule,
@@ -466,9 +481,11 @@ int serron_dropout_add_layer_norm(const void* input, const void* residual, int64
         SB_CHECK(eps >= 0.0 && std::isfinite(eps), name, ": eps must be finite and not negative, got ", eps);
         const Norm n = norm_of(name, outer, len, inner);
         const DropRule rule = drop_rule(name, p, seed, seed_device, sequence);
-        check_stats(name, mean, rstd);
+        check_stats(name, dtype, mean, rstd);
         if (n.numel() == 0) return;
         SB_CHECK(input && residual && sum && output, name, ": tensors must not be null");
+        check_elements(name, elem_size(dtype), input, residual, sum, output);
+        check_elements(name, elem_size(param_dtype), weight, bias);
         check_workspace(name, workspace, workspace_bytes, workspace_bytes_of(n, dtype, false));
         const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
         DeviceScope scope(device);

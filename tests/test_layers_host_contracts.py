@@ -38,3 +38,39 @@ def test_sizes_at_the_top_of_the_range(lib):
                 if outer * length * inner > ((1 << 63) - 1) // 64:
                     assert size(outer, length, inner, dtype, backward) == -1
                     assert "too many elements" in lib.serron_last_error().decode()
+
+
+def test_addresses_off_their_elements_are_refused(lib):
+    """A kernel that read them would fault; nothing is launched."""
+    def refused(rc, *patterns):
+        assert rc == _lib.ERR_INVALID
+        assert all(p in lib.serron_last_error().decode() for p in patterns)
+
+    elements = "tensors must start on a boundary of their elements"
+    space = 1 << 20
+    for size, dtype in ((4, 0), (8, 1), (2, 2), (2, 3)):
+        stat = 8 if dtype == 1 else 4
+        for k in range(6):
+            t = [64 + (size // 2 if i == k else 0) for i in range(4)] + [64 + (stat // 2 if i == k else 0) for i in (4, 5)]
+            refused(lib.serron_layer_norm(t[0], 2, 3, 4, dtype, t[1], t[2], dtype, 1e-5, t[3], t[4], t[5], 256, space, 0,
+                                          None), "serron::layer_norm: ", elements)
+            refused(lib.serron_layer_norm_backward(t[0], t[1], t[4], t[5], 2, 3, 4, dtype, t[2], dtype, t[3], None, None,
+                                                   256, space, 0, None), "serron::layer_norm_backward: ", elements)
+            refused(lib.serron_dropout_add_layer_norm(t[0], t[1], 2, 3, 4, dtype, None, None, dtype, 0.5, 1, None, 0, 1e-5,
+                                                      t[2], t[3], t[4], t[5], 256, space, 0, None),
+                    "serron::dropout_add_layer_norm: ", elements)
+            refused(lib.serron_dropout_add_layer_norm_backward(t[0], t[1], t[2], t[4], t[5], 2, 3, 4, dtype, t[3], dtype,
+                                                               0.5, 1, None, 0, 64, 64, None, None, 256, space, 0, None),
+                    "serron::dropout_add_layer_norm_backward: ", elements)
+        for k in range(3):
+            t = [64 + (size // 2 if i == k else 0) for i in range(3)]
+            refused(lib.serron_dropout(t[0], t[1], 12, 1, dtype, 0.5, 1, None, 0, t[2], 0, None), "serron::dropout: ",
+                    elements)
+    for k in range(2):  # gradients of float32 parameters beside 16-bit activations
+        t = [64 + (2 if i == k else 0) for i in range(2)]
+        refused(lib.serron_layer_norm_backward(64, 64, 64, 64, 2, 3, 4, 3, None, 0, 64, t[0], t[1], 256, space, 0, None),
+                elements)
+    refused(lib.serron_dropout(64, None, 12, 1, 0, 0.5, 1, 68, 0, 64, 0, None), "seed in device memory", "8 bytes")
+    # rows beyond the register kernels need a workspace
+    refused(lib.serron_layer_norm(64, 1, 300000, 1, 0, None, None, 0, 1e-5, 64, None, None, 264, 1 << 30, 0, None),
+            "serron::layer_norm: the workspace must be aligned to 256 bytes")
