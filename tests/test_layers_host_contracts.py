@@ -2,9 +2,16 @@
 
 from __future__ import annotations
 
+import os
+import shutil
+import subprocess
+
 import pytest
 
 from serron_b200 import _lib
+
+
+PACKAGE = os.path.dirname(os.path.abspath(_lib.__file__))
 
 
 @pytest.fixture(scope="module")
@@ -74,3 +81,10 @@ def test_addresses_off_their_elements_are_refused(lib):
     # rows beyond the register kernels need a workspace
     refused(lib.serron_layer_norm(64, 1, 300000, 1, 0, None, None, 0, 1e-5, 64, None, None, 264, 1 << 30, 0, None),
             "serron::layer_norm: the workspace must be aligned to 256 bytes")
+
+
+@pytest.mark.skipif(shutil.which("readelf") is None, reason="needs binutils")
+def test_binding_shares_the_cpp_runtime():
+    """A copy of its own beside torch's crashes where a number goes into an error message."""
+    out = subprocess.run(["readelf", "-d", os.path.join(PACKAGE, "_layers.so")], check=True, capture_output=True, text=True)
+    assert "[libstdc++.so.6]" in out.stdout
