@@ -88,3 +88,14 @@ def test_binding_shares_the_cpp_runtime():
     """A copy of its own beside torch's crashes where a number goes into an error message."""
     out = subprocess.run(["readelf", "-d", os.path.join(PACKAGE, "_layers.so")], check=True, capture_output=True, text=True)
     assert "[libstdc++.so.6]" in out.stdout
+
+
+@pytest.mark.skipif(shutil.which("make") is None, reason="needs make")
+def test_library_builds_without_torch(tmp_path):
+    """The C library has no torch symbols, and whoever builds it need have no torch."""
+    target = str(tmp_path / "_layers.so")
+    library = os.path.join(PACKAGE, "libserron_b200.so")
+    out = subprocess.run(["make", "-s", "-C", os.path.join(PACKAGE, "csrc"), "-o", library, f"LAYERS={target}",
+                          "PYTHON=false", target], capture_output=True, text=True)
+    assert out.returncode == 0 and not os.path.exists(target)
+    assert "_layers.so is not built: false has no torch" in out.stderr
