@@ -2,7 +2,8 @@
 
 The binding (``_layers.so``, from ``csrc/layer_binding.cpp``) allocates outputs and workspaces with torch's caching
 allocator, calls the C ABI on torch's current stream of the input's device and records the backward nodes, all
-outside Python.  What it cannot be handed is refused here: checks of tensors raise ``RuntimeError`` worded as the
+outside Python.  It registers the operators as ``torch.ops.serron.layer_norm``, ``dropout`` and
+``dropout_add_layer_norm``, which tracers, fake tensors and function transforms see.  What it cannot be handed is refused here: checks of tensors raise ``RuntimeError`` worded as the
 other operators' are, checks of numbers ``ValueError``.
 """
 
