@@ -307,13 +307,23 @@ SERRON_OPERATOR(dropout, dropout_kernel)
 SERRON_OPERATOR(_dropout_add_layer_norm, join_kernel)
 SERRON_OPERATOR(_dropout_add_layer_norm_backward, join_backward_kernel)
 
-// Gradients of a backward pass cannot be differentiated again: where a graph of them is asked for, its use is an error.
+// Gradients of a backward pass cannot be differentiated again: what asks for it, along whichever of `edges`, is an error.
 template <typename Tensors>
-void once(Tensors& grads) {
+void once(Tensors& grads, torch::autograd::edge_list&& edges) {
     const auto error = std::make_shared<torch::autograd::Error>(
-        "serron: a gradient of layer_norm or dropout_add_layer_norm is once_differentiable", torch::autograd::edge_list());
+        "serron: a gradient of layer_norm or dropout_add_layer_norm is once_differentiable", std::move(edges));
     for (const Tensor& g : grads)
         if (g.defined()) torch::autograd::set_history(g, error);
+}
+
+// The same for what a node computed while a graph of its gradients is recorded: they depend on its own inputs and on those
+// that came to it.
+void once_from(const Node& node, const variable_list& came, variable_list& grads) {
+    if (!at::GradMode::is_enabled()) return;
+    torch::autograd::edge_list edges = node.next_edges();
+    for (const Tensor& g : came)
+        if (g.defined()) edges.push_back(torch::autograd::impl::gradient_edge(g));
+    once(grads, std::move(edges));
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -330,7 +340,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_backward_autograd(const Tensor& grad_out
     }
     const Tensor w = given(weight);
     if (torch::autograd::compute_requires_grad(grad_output, input, w))
-        once(out);
+        once(out, torch::autograd::collect_next_edges(grad_output, input, w));
     return {out[0], out[1], out[2]};
 }
 
@@ -355,7 +365,7 @@ struct LayerNormBackward : public Node {
         std::tie(out[0], out[1], out[2]) = _layer_norm_backward().call(
             grads[0], input, stats.unpack(), w.defined() ? MaybeTensor(w) : MaybeTensor(), dim, params,
             {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2)});
-        if (at::GradMode::is_enabled()) once(out);
+        once_from(*this, grads, out);
         return out;
     }
 };
@@ -455,7 +465,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> join_backward_autograd(
     }
     const Tensor gh = given(grad_sum), w = given(weight);
     if (torch::autograd::compute_requires_grad(grad_output, gh, sum, w))
-        once(out);
+        once(out, torch::autograd::collect_next_edges(grad_output, gh, sum, w));
     return {out[0], out[1], out[2], out[3]};
 }
 
@@ -486,7 +496,7 @@ struct DropoutAddLayerNormBackward : public Node {
             key.defined() ? MaybeTensor(key) : MaybeTensor(), rule.sequence,
             {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2),
              task_should_compute_output(3)});
-        if (at::GradMode::is_enabled()) once(out);
+        once_from(*this, grads, out);
         return out;
     }
 };

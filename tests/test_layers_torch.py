@@ -208,6 +208,30 @@ def test_function_transforms(layers, name):
         _close(g, torch.func.grad(lambda x: plain(x, *args[1:]).sin().sum())(x))
 
 
+@pytest.mark.parametrize("name", ["layer_norm", "join"])
+def test_second_derivatives_are_refused(layers, name):
+    """However they are asked for: neither zero nor part of one comes back."""
+    f, _ = _functions(layers)[name]
+    if name == "layer_norm":
+        f = lambda x, r, w, b: layers.layer_norm(x, w, b, 1, EPS)  # noqa: E731
+    x, r, w, b = _tensors((3, 5, 4), 1)
+    leaf = x.clone().requires_grad_()
+    g = torch.autograd.grad(f(leaf, r, w, b).square().sum(), leaf, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        torch.func.grad(lambda v: torch.func.grad(lambda x: f(x, r, w, b).sin().sum())(v).sin().sum())(x)
+    for leaf in (x.clone().requires_grad_(), x.transpose(0, 1)[..., ::2].requires_grad_()):  # the second one is copied
+        v = r if leaf.shape == r.shape else r.transpose(0, 1)[..., ::2]
+        g = torch.autograd.grad(f(leaf, v, None, None).sum(), leaf, create_graph=True)[0]
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            torch.autograd.grad((g * leaf).sum(), leaf)  # it reaches the leaf by another way too
+    y = f(x, r, w.requires_grad_(), b)
+    gy = torch.ones_like(y, requires_grad=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        torch.autograd.grad(torch.autograd.grad(y, w, gy, create_graph=True)[0].sum(), gy)
+
+
 def test_dropout_is_linear_in_its_gradient(layers):
     """Its backward pass is dropout again, with all of its derivatives."""
     x, r, *_ = _tensors((3, 5, 4), 1)
