@@ -307,6 +307,14 @@ SERRON_OPERATOR(dropout, dropout_kernel)
 SERRON_OPERATOR(_dropout_add_layer_norm, join_kernel)
 SERRON_OPERATOR(_dropout_add_layer_norm_backward, join_backward_kernel)
 
+// There are no forward-mode derivatives; an output without a tangent would stand for one of zero.
+template <typename... T>
+void refuse_tangents(const char* name, const T&... inputs) {
+    const auto has = [](const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); };
+    TORCH_CHECK_NOT_IMPLEMENTED(!(has(inputs) || ...), "serron::", name,
+                                ": an input carries a tangent, and there is no forward-mode derivative");
+}
+
 // Gradients of a backward pass cannot be differentiated again: what asks for it, along whichever of `edges`, is an error.
 template <typename Tensors>
 void once(Tensors& grads, torch::autograd::edge_list&& edges) {
@@ -332,6 +340,7 @@ void once_from(const Node& node, const variable_list& came, variable_list& grads
 std::tuple<Tensor, Tensor, Tensor> norm_backward_autograd(const Tensor& grad_output, const Tensor& input,
                                                           const Tensor& stats, const MaybeTensor& weight, int64_t dim,
                                                           at::ScalarType params, std::array<bool, 3> wanted) {
+    refuse_tangents("layer_norm_backward", grad_output, input, given(weight));
     std::array<Tensor, 3> out;
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -372,6 +381,7 @@ struct LayerNormBackward : public Node {
 
 Tensor norm_autograd(const Tensor& input, const MaybeTensor& weight, const MaybeTensor& bias, int64_t dim, double eps) {
     const Tensor given_w = given(weight), given_b = given(bias);
+    refuse_tangents("layer_norm", input, given_w, given_b);
     const bool records = torch::autograd::compute_requires_grad(input, given_w, given_b);
     Tensor x = input, y, stats;
     {
@@ -433,6 +443,7 @@ struct DropoutBackward : public Node {
 Tensor dropout_autograd(const Tensor& input, const MaybeTensor& residual, int64_t span, double p, int64_t seed,
                         const MaybeTensor& seed_tensor, int64_t sequence) {
     const Tensor given_r = given(residual);
+    refuse_tangents("dropout", input, given_r);
     const bool records = torch::autograd::compute_requires_grad(input, given_r);
     Tensor y;
     {
@@ -457,6 +468,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> join_backward_autograd(
     const Tensor& grad_output, const MaybeTensor& grad_sum, const Tensor& sum, const Tensor& stats,
     const MaybeTensor& weight, int64_t dim, at::ScalarType params, double p, int64_t seed, const MaybeTensor& seed_tensor,
     int64_t sequence, std::array<bool, 4> wanted) {
+    refuse_tangents("dropout_add_layer_norm_backward", grad_output, given(grad_sum), sum, given(weight));
     std::array<Tensor, 4> out;
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -505,6 +517,7 @@ std::tuple<Tensor, Tensor> join_autograd(const Tensor& input, const Tensor& resi
                                          const MaybeTensor& bias, double p, int64_t seed, const MaybeTensor& seed_tensor,
                                          int64_t sequence, int64_t dim, double eps) {
     const Tensor given_w = given(weight), given_b = given(bias);
+    refuse_tangents("dropout_add_layer_norm", input, residual, given_w, given_b);
     const bool records = torch::autograd::compute_requires_grad(input, residual, given_w, given_b);
     Tensor y, h, stats;
     {

@@ -9,7 +9,8 @@ same bits.  The reconstructions run on the library's fixed-point solver instead 
 
 ``layer_norm``, ``dropout`` and ``dropout_add_layer_norm`` are what a network puts around the learnable
 layers; the reference has no counterpart.  They compute in float32 (float64 for float64 inputs) and return the
-input's dtype, so autocast leaves them as they are.  The gradients of the norms cannot be differentiated again.
+input's dtype, so autocast leaves them as they are.  The gradients of the norms cannot be differentiated again, and there
+are no forward-mode derivatives: both are errors.
 """
 
 from __future__ import annotations

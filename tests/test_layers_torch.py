@@ -232,6 +232,34 @@ def test_second_derivatives_are_refused(layers, name):
         torch.autograd.grad(torch.autograd.grad(y, w, gy, create_graph=True)[0].sum(), gy)
 
 
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("which", range(4))
+def test_forward_mode_is_refused(layers, name, which):
+    """There are no forward-mode derivatives, and an output without a tangent would pass for a constant."""
+    f, _ = _functions(layers)[name]
+    args = list(_tensors((3, 5, 4), 1))
+    if (name, which) in (("layer_norm", 1), ("dropout", 2), ("dropout", 3)):
+        return  # not an argument of the operator
+    with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+        torch.func.jvp(lambda v: f(*args[:which], v, *args[which + 1:]), (args[which],), (torch.ones_like(args[which]),))
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        args[which] = torch.autograd.forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+            f(*args)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tangents_of_gradients_are_refused(layers, name):
+    """Forward over reverse: the gradient that comes to a node carries the tangent."""
+    f, _ = _functions(layers)[name]
+    x, r, w, b = (t.requires_grad_() for t in _tensors((3, 5, 4), 1))
+    y = f(x, r, w, b)
+    with torch.autograd.forward_ad.dual_level():
+        gy = torch.autograd.forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+            torch.autograd.grad(y, x, gy)
+
+
 def test_dropout_is_linear_in_its_gradient(layers):
     """Its backward pass is dropout again, with all of its derivatives."""
     x, r, *_ = _tensors((3, 5, 4), 1)
