@@ -135,6 +135,11 @@ void check_params(const char* name, const Tensor& x, int64_t dim, const Tensor& 
                 ": weight and bias must share a dtype");
 }
 
+void check_param_type(const char* name, const Tensor& weight, at::ScalarType params) {
+    TORCH_CHECK(!weight.defined() || weight.scalar_type() == params, "serron::", name, ": a weight of ", params,
+                " is needed, got ", weight.scalar_type());
+}
+
 void check_seed(const char* name, const Tensor& x, const Tensor& seed) {
     if (!seed.defined()) return;
     TORCH_CHECK(seed.device() == x.device(), "serron::", name, ": all tensors must be on one device");
@@ -205,6 +210,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_backward_kernel(const Tensor& grad_outpu
     const Layout l = layout_of(x, dim);
     const Tensor gy = like(grad_output, x), w = plain(weight), s = checked_stats(name, stats, x, l);
     check_params(name, x, dim, w, Tensor());
+    check_param_type(name, w, params);
     std::array<Tensor, 3> out;
     if (wanted[0]) out[0] = at::empty_like(x);
     for (const int i : {1, 2})
@@ -272,6 +278,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> join_backward_kernel(
     check_beside(name, gy, h);
     if (gh.defined()) check_beside(name, gh, h);
     check_params(name, h, dim, w, Tensor());
+    check_param_type(name, w, params);
     check_seed(name, h, key);
     std::array<Tensor, 4> out;
     for (const int i : {0, 1})
@@ -355,6 +362,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_backward_autograd(const Tensor& grad_out
 
 struct LayerNormBackward : public Node {
     SavedVariable x, weight, stats;
+    c10::SmallVector<int64_t, 8> strides;  // of x: the statistics lie in the order of its memory
     int64_t dim = 0;
     at::ScalarType params = at::kFloat;
 
@@ -370,7 +378,11 @@ struct LayerNormBackward : public Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(3);
         if (!grads[0].defined()) return out;
-        const Tensor input = x.unpack(), w = weight.unpack();
+        Tensor input = x.unpack();
+        const Tensor w = weight.unpack();
+        // hooks on saved tensors (as to keep them on the host) may bring x back in another order
+        if (input.strides() != at::IntArrayRef(strides))
+            input = at::empty_strided(input.sizes(), strides, input.options()).copy_(input);
         std::tie(out[0], out[1], out[2]) = _layer_norm_backward().call(
             grads[0], input, stats.unpack(), w.defined() ? MaybeTensor(w) : MaybeTensor(), dim, params,
             {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2)});
@@ -395,6 +407,7 @@ Tensor norm_autograd(const Tensor& input, const MaybeTensor& weight, const Maybe
         node->x = SavedVariable(x, false);
         node->weight = SavedVariable(given_w, false);
         node->stats = SavedVariable(stats, false);
+        node->strides = c10::SmallVector<int64_t, 8>(x.strides().begin(), x.strides().end());
         node->dim = dim;
         node->params = param_type(x, given_w, given_b);
         torch::autograd::set_history(y, node);

@@ -69,3 +69,28 @@ def test_longest_dimension(serron, inner):
             if inner == 1:
                 _near(grads[1], lambda s: gc[s].float() * (xc[s].float() - m) * rstd, 3 * chain)
                 assert torch.equal(grads[2], gc)
+
+
+def _rand(shape, dtype, seed):
+    gen = torch.Generator("cuda").manual_seed(seed)
+    return torch.randn(shape, generator=gen, device="cuda").to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("name", ["rows", "channels_last", "transposed"])
+def test_saved_tensors_kept_on_the_host(serron, name, dtype):
+    """save_on_cpu packs into row-major memory; gradients are those without it, to the bit."""
+    base = _rand((3, 24, 6, 10), dtype, 1)
+    x = {"rows": base, "channels_last": base.to(memory_format=torch.channels_last),
+         "transposed": base.permute(3, 1, 0, 2).contiguous().permute(2, 1, 3, 0)}[name]
+    w, b, r, gy, gh = _rand((24,), torch.float32, 2), _rand((24,), torch.float32, 3), *(_rand(x.shape, dtype, k) for k in (4, 5, 6))
+    leaves = [t.requires_grad_() for t in (x, r, w, b)]
+    calls = [lambda: (serron.layer_norm(x, w, b),), lambda: (serron.dropout(x, 0.3, seed=torch.tensor(5, device="cuda")),),
+             lambda: serron.dropout_add_layer_norm(x, r, w, b, p=0.3, seed=5)]
+    for call in calls:
+        want = torch.autograd.grad(call(), leaves, (gy, gh)[:len(call())], allow_unused=True)
+        with torch.autograd.graph.save_on_cpu(pin_memory=True):
+            outputs = call()
+        got = torch.autograd.grad(outputs, leaves, (gy, gh)[:len(outputs)], allow_unused=True)
+        for a, c in zip(got, want):
+            assert a is c is None or torch.equal(a, c)

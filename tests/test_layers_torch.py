@@ -293,6 +293,9 @@ def test_views_with_a_pending_sign_or_conjugation(layers):
     (lambda o, x, w: o.layer_norm(x, torch.ones(5, dtype=x.dtype), None, 1, EPS), "one device"),
     (lambda o, x, w: o._layer_norm_backward(x[:1], x, w, None, 1, w.dtype, [True] * 3), "shape and dtype"),
     (lambda o, x, w: o._layer_norm_backward(x, x, w, None, 1, w.dtype, [True] * 3), "statistics of another input"),
+    (lambda o, x, w: o._layer_norm_backward(x, x, x.new_empty(2, 12), w.float(), 1, w.dtype, [True] * 3), "weight of"),
+    (lambda o, x, w: o._dropout_add_layer_norm_backward(x, None, x, x.new_empty(2, 12), w, 1, torch.float32, 0.3, 7, None,
+                                                        2, [True] * 4), "weight of"),
     (lambda o, x, w: o.dropout(x, x[:1], 1, 0.3, 7, None, 2), "shape and dtype"),
     (lambda o, x, w: o.dropout(x, None, 1, 0.3, 7, w, 2), "one int64"),
     (lambda o, x, w: o.dropout_add_layer_norm(x, x.float(), None, None, 0.3, 7, None, 2, 1, EPS), "shape and dtype"),
@@ -313,3 +316,45 @@ def test_no_kernel_for_cpu_tensors():
         torch.ops.serron.layer_norm(x, None, None, 1, EPS)
     with pytest.raises(NotImplementedError, match="CPU"):
         torch.ops.serron.dropout(x, None, 1, 0.3, 7, None, 2)
+
+
+HOOKS = {
+    "contiguous": lambda t: t.contiguous(),
+    "reversed": lambda t: t.permute(*reversed(range(t.dim()))).contiguous().permute(*reversed(range(t.dim()))),
+    "strided": lambda t: torch.stack((t, t + 1), -1)[..., 0],
+}
+
+
+@pytest.mark.parametrize("hook", HOOKS)
+@pytest.mark.parametrize("order", [(0, 1, 2, 3), (0, 2, 3, 1), (3, 0, 1, 2)])
+def test_hooks_may_bring_saved_tensors_back_in_another_order(layers, order, hook):
+    """What a hook returns has the values of what it was given, and not its strides (torch's save_on_cpu packs into
+    row-major memory)."""
+    shape = (2, 3, 4, 5)
+    memory, other, w, b = _tensors([shape[d] for d in order], order.index(1))
+    x = memory.permute(*[order.index(d) for d in range(4)])
+    r = other.reshape(shape)
+    assert x.shape == shape
+    for name in NAMES:
+        f, _ = _functions(layers)[name]
+        leaves = [t.detach().requires_grad_() for t in (x, r, w, b)]
+        want = torch.autograd.grad(f(*leaves).sin().sum(), leaves, allow_unused=True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, HOOKS[hook]):
+            y = f(*leaves).sin().sum()
+        for a, c in zip(torch.autograd.grad(y, leaves, allow_unused=True), want):
+            assert (a is None) == (c is None)
+            if a is not None:
+                _close(a, c)
+
+
+@pytest.mark.parametrize("change", [lambda t: t.float(), lambda t: t[:1]])
+def test_hooks_that_change_a_saved_tensor_are_refused(layers, change):
+    """Another dtype or size would be read past its end."""
+    x, r, w, b = _tensors((3, 5, 4), 1)
+    leaf, w = x.to("meta").requires_grad_(), w.to("meta")
+    for f in (lambda: layers.layer_norm(leaf, w, None, 1, EPS),
+              lambda: layers.dropout_add_layer_norm(leaf, leaf, w, None, 0.3, 7, None, 2, 1, EPS)[0]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            y = f()
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, leaf, torch.empty_like(y))
