@@ -513,12 +513,22 @@ struct DropoutAddLayerNormBackward : public Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(4);
         if (!grads[0].defined() && !grads[1].defined()) return out;
-        const Tensor h = sum.unpack(shared_from_this()), w = weight.unpack(), key = seed.unpack();
-        const Tensor gy = grads[0].defined() ? grads[0] : at::zeros_like(h);
+        const Tensor key = seed.unpack();
+        const MaybeTensor seed_tensor = key.defined() ? MaybeTensor(key) : MaybeTensor();
+        if (!grads[0].defined()) {
+            // the norm's output was not used: what it would be at this input, finite or not, is in no gradient
+            if (task_should_compute_output(0))
+                out[0] = dropout().call(grads[1], std::nullopt, 1, rule.p, rule.seed, seed_tensor, rule.sequence);
+            if (task_should_compute_output(1)) out[1] = grads[1];
+            for (const int i : {2, 3})
+                if (task_should_compute_output(i))
+                    out[i] = at::zeros({grads[1].size(dim)}, grads[1].options().dtype(params));
+            return out;
+        }
+        const Tensor h = sum.unpack(shared_from_this()), w = weight.unpack();
         std::tie(out[0], out[1], out[2], out[3]) = _dropout_add_layer_norm_backward().call(
-            gy, grads[1].defined() ? MaybeTensor(grads[1]) : MaybeTensor(), h, stats.unpack(),
-            w.defined() ? MaybeTensor(w) : MaybeTensor(), dim, params, rule.p, rule.seed,
-            key.defined() ? MaybeTensor(key) : MaybeTensor(), rule.sequence,
+            grads[0], grads[1].defined() ? MaybeTensor(grads[1]) : MaybeTensor(), h, stats.unpack(),
+            w.defined() ? MaybeTensor(w) : MaybeTensor(), dim, params, rule.p, rule.seed, seed_tensor, rule.sequence,
             {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2),
              task_should_compute_output(3)});
         once_from(*this, grads, out);

@@ -6,6 +6,8 @@ from __future__ import annotations
 import pytest
 import torch
 
+from tests import layer_oracle as oracle
+
 pytestmark = pytest.mark.gpu
 
 
@@ -94,3 +96,16 @@ def test_saved_tensors_kept_on_the_host(serron, name, dtype):
         got = torch.autograd.grad(outputs, leaves, (gy, gh)[:len(outputs)], allow_unused=True)
         for a, c in zip(got, want):
             assert a is c is None or torch.equal(a, c)
+
+
+@pytest.mark.parametrize("shape", [(12, 96), (3, 1001), (2, 10, 6, 6), (2, 10, 5, 5)])
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.float16])
+def test_an_unused_norm_has_no_part_in_gradients(serron, shape, dtype):
+    """Rows that hold NaN or an infinity, and rows without spread at eps = 0, have no norm; the sum's gradient passes by."""
+    x, r, gh = (_rand(shape, dtype, k) for k in (1, 2, 3))
+    x.view(-1)[5], r.view(-1)[-1] = float("inf"), float("nan")
+    leaves = [x.requires_grad_(), r.requires_grad_(), *(_rand((shape[1],), dtype, k).requires_grad_() for k in (4, 5))]
+    _, h = serron.dropout_add_layer_norm(*leaves, p=0.3, seed=7, sequence=2, eps=0.0)
+    gx, gr, gw, gb = torch.autograd.grad(h, leaves, gh)
+    assert torch.equal(gx, oracle.dropout(gh, 0.3, 7, 2)) and torch.equal(gr, gh)
+    assert not gw.any() and not gb.any()

@@ -358,3 +358,15 @@ def test_hooks_that_change_a_saved_tensor_are_refused(layers, change):
             y = f()
         with pytest.raises(RuntimeError):
             torch.autograd.grad(y, leaf, torch.empty_like(y))
+
+
+def test_an_unused_norm_has_no_part_in_gradients(layers):
+    """A row that holds an infinity has no norm, and the sum's gradient passes it by where only the sum is used."""
+    x, r, w, b = _tensors((3, 5, 4), 1)
+    x[0, 2, 1], r[1, 0, 0] = float("inf"), float("nan")
+    leaves = [t.requires_grad_() for t in (x, r, w, b)]
+    _, h = layers.dropout_add_layer_norm(*leaves, 0.3, 7, None, 2, 1, EPS)
+    gh = torch.randn_like(h)
+    gx, gr, gw, gb = torch.autograd.grad(h, leaves, gh, create_graph=True)
+    assert torch.equal(gx, layer_oracle.dropout(gh, 0.3, 7, 2)) and torch.equal(gr, gh)
+    assert not gw.any() and not gb.any()
