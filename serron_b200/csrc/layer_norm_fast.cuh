@@ -452,12 +452,13 @@ __global__ void __maxnreg__(128) norm_columns_bwd_kernel(const __grid_constant__
         }
         column_totals<V, 2>(s, shared, phase);
         if (live && stores) {
-            // dx = rstd (g w - mean(g w) - xhat mean(g w xhat)), with rstd multiplied into what is the same for a row
+            // dx = rstd (g w - mean(g w) - xhat mean(g w xhat)), with xhat's rstd multiplied into the mean, which is the same
+            // for a row; rstd^2 would leave float32's range for rows of tiny spread, whose dx does not
             F scale, shift;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                shift.e[i] = mul(mul(s[0].e[i], splat<E>(-inverse)), rstd.e[i]);
-                scale.e[i] = mul(mul(s[1].e[i], splat<E>(-inverse)), mul(rstd.e[i], rstd.e[i]));
+                shift.e[i] = mul(s[0].e[i], splat<E>(-inverse));
+                scale.e[i] = mul(mul(s[1].e[i], splat<E>(-inverse)), rstd.e[i]);
             }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
@@ -466,8 +467,8 @@ __global__ void __maxnreg__(128) norm_columns_bwd_kernel(const __grid_constant__
                     F d;
 #pragma unroll
                     for (int i = 0; i < N; ++i)
-                        d.e[i] = fma(mul(g.e[i], splat<E>(w[k])), rstd.e[i],
-                                     fma(sub(h.e[i], mean.e[i]), scale.e[i], shift.e[i]));
+                        d.e[i] = mul(fma(sub(h.e[i], mean.e[i]), scale.e[i], fma(g.e[i], splat<E>(w[k]), shift.e[i])),
+                                     rstd.e[i]);
                     store_dx<T, V, JOIN>(d, first + k * step, a, extra[JOIN ? k : 0], keys);
                 }
             }
@@ -917,14 +918,14 @@ __global__ void __maxnreg__(128) norm_rows_bwd_kernel(const __grid_constant__ No
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
                         if (r < rows) {
-                            const E shift = splat<E>(-s[2 * r] * inverse * rstd[r]);
-                            const E scale = splat<E>(-s[2 * r + 1] * inverse * (rstd[r] * rstd[r]));
+                            const E shift = splat<E>(-s[2 * r] * inverse);
+                            const E scale = splat<E>(-s[2 * r + 1] * inverse * rstd[r]);
                             const F g = gy[r][k].floats(), h = x[r][k].floats();
                             F d;
 #pragma unroll
                             for (int i = 0; i < N; ++i)
-                                d.e[i] = fma(mul(g.e[i], wk.e[i]), splat<E>(rstd[r]),
-                                             fma(sub(h.e[i], splat<E>(mean[r])), scale, shift));
+                                d.e[i] = mul(fma(sub(h.e[i], splat<E>(mean[r])), scale, fma(g.e[i], wk.e[i], shift)),
+                                             splat<E>(rstd[r]));
                             store_dx<T, V, JOIN>(d, base + r * row_step + k * place.all * V, a, extra[JOIN ? r : 0][k],
                                                  keys, place.whole(j), place.lo(j), place.hi(j));
                         }

@@ -109,3 +109,38 @@ def test_an_unused_norm_has_no_part_in_gradients(serron, shape, dtype):
     gx, gr, gw, gb = torch.autograd.grad(h, leaves, gh)
     assert torch.equal(gx, oracle.dropout(gh, 0.3, 7, 2)) and torch.equal(gr, gh)
     assert not gw.any() and not gb.any()
+
+
+def _scaled_signs(shape, dim, dtype, scale):
+    """Signs of equal number in every row (a zero beside them where the length is odd), times a power of two."""
+    length = shape[dim]
+    row = torch.cat((torch.ones(length // 2), -torch.ones(length // 2), torch.zeros(length % 2)))
+    moved = [s for d, s in enumerate(shape) if d != dim]
+    return (row * scale).expand(*moved, length).movedim(-1, dim).contiguous().to("cuda", dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [2.0**-65, 2.0**-63, 2.0**50])
+@pytest.mark.parametrize("shape,dim", [((9, 96), 1), ((9, 97), 1), ((40, 1024), 1), ((3, 20001), 1), ((2, 70000), 1),
+                                       ((2, 24, 6, 6), 1), ((2, 24, 5, 7), 1), ((1, 1500, 2, 4), 1), ((1, 2100, 3, 3), 1)])
+def test_gradients_of_any_spread(serron, shape, dim, scale, dtype):
+    """rstd is up to 2^65, its square beyond float32; no term of the formula is.  Sums and squares of the signs are exact; the
+    variance, 2^-130, is rounded to a multiple of 2^-149, which takes 2^-20 of it and 2^-21 of rstd, a 64th of the bounds'
+    K u.  So those hold as at any scale."""
+    x, r = _scaled_signs(shape, dim, dtype, scale), torch.zeros(shape, dtype=dtype, device="cuda")
+    w, b = 1 + 0.3 * _rand((shape[dim],), torch.float32, 1), _rand((shape[dim],), torch.float32, 2)
+    gy, gh = _rand(shape, dtype, 3), _rand(shape, torch.float32, 4) / scale
+    leaves = [t.requires_grad_() for t in (x, r, w, b)]
+    ref = oracle.Norm(x.detach(), w.detach(), b.detach(), dim, 0.0)
+    y = serron.layer_norm(x, w, b, dim=dim, eps=0.0)
+    with torch.no_grad():
+        oracle.within(y, ref.y, ref.y_bound(), "y")
+    grads = torch.autograd.grad(y, (x, w, b), gy)
+    for name, got, (want, bound) in zip(("dx", "dw", "db"), grads, ref.backward(gy)):
+        oracle.within(got, want, bound, name)
+    gh = gh.to(dtype)
+    outputs = serron.dropout_add_layer_norm(x, r, w, b, p=0.0, seed=0, dim=dim, eps=0.0)
+    grads = torch.autograd.grad(outputs, leaves, (gy, gh))
+    (want, bound), *_ = ref.backward(gy, gh)
+    for got in grads[:2]:
+        oracle.within(got, want, bound, "dx of the join")
