@@ -61,11 +61,12 @@ __device__ __forceinline__ E quotient(E s, float n, float inverse) {
     return fma(fma(splat<E>(-n), q, s), splat<E>(inverse), q);
 }
 
-// 1 / sqrt(v): the approximation and one Newton step (infinite v: zero, as 1 / sqrt gives).
+// 1 / sqrt(v): the approximation and one step of Newton's iteration.  The step has 0 * infinity in it at zero and at
+// infinity, where the approximation is exact (infinity and zero).
 __device__ __forceinline__ float root_inverse(float v) {
     const float r = rsqrtf(v);
     const float better = fmaf(r * 0.5f, fmaf(-(v * r), r, 1.0f), r);
-    return v < __int_as_float(0x7f800000) ? better : r;
+    return better == better ? better : r;
 }
 
 // What the kernels are compiled for: the norm alone, or the join with the generator's keys as operands in constant memory

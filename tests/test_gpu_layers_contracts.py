@@ -144,3 +144,22 @@ def test_gradients_of_any_spread(serron, shape, dim, scale, dtype):
     (want, bound), *_ = ref.backward(gy, gh)
     for got in grads[:2]:
         oracle.within(got, want, bound, "dx of the join")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize("shape,dim", [((9, 96), 1), ((9, 97), 1), ((40, 1024), 1), ((2, 20000), 1), ((2, 140000), 1),
+                                       ((2, 24, 6, 6), 1), ((2, 24, 5, 7), 1), ((1, 2100, 3, 3), 1)])
+def test_statistics_of_no_variance(serron, shape, dim, dtype):
+    """eps = 0: rstd is 1 / 0, an infinity, of every kernel; what is off the mean by less than squares can hold becomes an
+    infinity with its sign, what is not off it is 0 / 0.  With eps it is finite."""
+    tiny = 2.0**-80 if dtype != torch.float64 else 2.0**-600
+    x = _scaled_signs(shape, dim, dtype, tiny)
+    y = serron.layer_norm(x, dim=dim, eps=0.0)
+    assert torch.equal(y.nan_to_num(0.0, posinf=1.0, neginf=-1.0), (x / tiny)) and torch.equal(y.isnan(), x == 0)
+    level = torch.full(shape, 3.0, dtype=dtype, device="cuda")
+    assert bool(serron.layer_norm(level, dim=dim, eps=0.0).isnan().all())
+    assert not serron.layer_norm(level, dim=dim).any()
+    _, stats = torch.ops.serron._layer_norm(level, None, None, dim, 0.0, True)
+    assert bool((stats[0] == 3.0).all()) and bool((stats[1] == float("inf")).all())
+    huge = _scaled_signs(shape, dim, dtype, 2.0**70 if dtype != torch.float64 else 2.0**600)  # an infinite variance: rstd 0
+    assert not serron.layer_norm(huge, dim=dim, eps=0.0).any()
