@@ -75,8 +75,8 @@ void launch_dropout(const char* name, const void* x_, const void* residual_, voi
     if constexpr (!std::is_same_v<T, double>) {
         constexpr int V = 16 / sizeof(T), U = kDropVectors;
         const bool wide = aligned(x, 16) && aligned(residual, 16) && aligned(y, 16);
-        if (rule.all) span = n;  // one decision for everything
-        if (span == 1 && wide) {
+        if (rule.all) span = n;  // one decision for everything, which the kernels of a span look up in the rule
+        if (span == 1 && wide && !rule.all) {
             const unsigned blocks = grid_of(name, ceil_div64(n, 256 * U * V));
             auto kernel = rule.seed_device
                               ? (residual ? dropout_kernel<T, V, U, true, true> : dropout_kernel<T, V, U, false, true>)

@@ -163,3 +163,18 @@ def test_statistics_of_no_variance(serron, shape, dim, dtype):
     assert bool((stats[0] == 3.0).all()) and bool((stats[1] == float("inf")).all())
     huge = _scaled_signs(shape, dim, dtype, 2.0**70 if dtype != torch.float64 else 2.0**600)  # an infinite variance: rstd 0
     assert not serron.layer_norm(huge, dim=dim, eps=0.0).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.float16, torch.bfloat16])
+def test_everything_is_dropped_whatever_the_words(serron, dtype):
+    """The first word of this seed is 2^32 - 1, which no threshold in 32 bits is above."""
+    seed = 1352247272
+    assert oracle.philox(oracle.np.zeros(1, dtype="uint64"), 0, seed)[0, 0] == 0xFFFFFFFF
+    for n in (1, 2, 7, 300):
+        x = torch.full((n,), float("nan"), dtype=dtype, device="cuda")
+        r = _rand((n,), dtype, 1)
+        for given in (seed, torch.tensor(seed, device="cuda")):
+            for unit in ("element", "sample"):
+                assert not serron.dropout(x, 1.0, seed=given, unit=serron.DropoutUnit(unit)).any()
+                assert torch.equal(serron.dropout(x, 1.0, seed=given, residual=r, unit=serron.DropoutUnit(unit)), r)
+            assert torch.equal(serron.dropout_add_layer_norm(x, r, p=1.0, seed=given, dim=0)[1], r)
