@@ -86,35 +86,52 @@ class LayerNorm2d(nn.Module):
         return F.layer_norm(x, self.weight, self.bias, eps=self.eps)
 
 
-def _draw_seed() -> int:
+def _draw_seed(x: torch.Tensor) -> int:
     """A seed from torch's CPU generator: ``torch.manual_seed`` repeats it, and recomputing a layer under restored
-    generator states (activation checkpointing) draws the same mask."""
+    generator states (activation checkpointing) draws the same mask.  A CUDA graph would keep it for all of its replays."""
+    if x.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("serron: a dropout layer that draws its own seed would drop the same elements in every replay of "
+                           "a captured CUDA graph; pass it seed= as an int64 tensor on the GPU and change that between replays")
     return int(torch.randint(0, (1 << 63) - 1, (), dtype=torch.int64))
 
 
 class Dropout(nn.Module):
-    """Dropout of elements, channels or samples while training, and the sum with a residual where one is given."""
+    """Dropout of elements, channels or samples while training, and the sum with a residual where one is given.
+
+    Every call draws a seed of its own, unless it is given ``seed`` (and ``sequence``) as :func:`functional.dropout` takes
+    them: a captured CUDA graph needs a seed in a tensor, and layers that share it a ``sequence`` each.
+    """
 
     def __init__(self, p: float = 0.5, *, unit: DropoutUnit = DropoutUnit.ELEMENT) -> None:
         super().__init__()
         self.p = p
         self.unit = unit
 
-    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, *,
+                seed: int | torch.Tensor | None = None, sequence: int = 0) -> torch.Tensor:
         if not self.training or self.p == 0.0:
             return x if residual is None else x + residual
-        return F.dropout(x, self.p, seed=_draw_seed(), unit=self.unit, residual=residual)
+        return F.dropout(x, self.p, seed=_draw_seed(x) if seed is None else seed, sequence=sequence, unit=self.unit,
+                         residual=residual)
 
 
 class DropoutAddLayerNorm2d(LayerNorm2d):
-    """``(layer_norm(h), h)`` with ``h = residual + dropout(x)``; nothing is dropped outside training."""
+    """``(layer_norm(h), h)`` with ``h = residual + dropout(x)``; nothing is dropped outside training.
+
+    Seeds are drawn or given as in :class:`Dropout`.
+    """
 
     def __init__(self, channels: int, p: float = 0.5, *, eps: float = 1e-5, affine: bool = True,
                  dtype: torch.dtype = torch.float32, device: torch.device | str | None = None) -> None:
         super().__init__(channels, eps=eps, affine=affine, dtype=dtype, device=device)
         self.p = p
 
-    def forward(self, x: torch.Tensor, residual: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-        drops = self.training and self.p > 0.0
-        return F.dropout_add_layer_norm(x, residual, self.weight, self.bias, p=self.p if drops else 0.0,
-                                        seed=_draw_seed() if drops else 0, eps=self.eps)
+    def forward(self, x: torch.Tensor, residual: torch.Tensor, *, seed: int | torch.Tensor | None = None,
+                sequence: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+        p = self.p if self.training else 0.0
+        if p == 0.0:
+            seed, sequence = 0, 0
+        elif seed is None:
+            seed = _draw_seed(x)
+        return F.dropout_add_layer_norm(x, residual, self.weight, self.bias, p=p, seed=seed, sequence=sequence,
+                                        eps=self.eps)

@@ -178,3 +178,37 @@ def test_everything_is_dropped_whatever_the_words(serron, dtype):
                 assert not serron.dropout(x, 1.0, seed=given, unit=serron.DropoutUnit(unit)).any()
                 assert torch.equal(serron.dropout(x, 1.0, seed=given, residual=r, unit=serron.DropoutUnit(unit)), r)
             assert torch.equal(serron.dropout_add_layer_norm(x, r, p=1.0, seed=given, dim=0)[1], r)
+
+
+def test_layers_take_their_seed_from_memory_in_a_graph(serron):
+    """Replays drop what the seed in the tensor says, forward and backward, as the functions do without a graph."""
+    x, r, gy, gh = (_rand((2, 6, 9, 9), torch.float32, k) for k in range(4))
+    leaves = [t.requires_grad_() for t in (x, r)]
+    drop = serron.Dropout(0.5, unit=serron.DropoutUnit.CHANNEL)
+    join = serron.DropoutAddLayerNorm2d(6, 0.5, device="cuda")
+    seed = torch.zeros(1, dtype=torch.int64, device="cuda")
+
+    def step(seed):
+        y, h = join(drop(x, seed=seed, sequence=1), r, seed=seed, sequence=2)
+        return y, h, *torch.autograd.grad((y, h), (*leaves, join.weight, join.bias), (gy, gh))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(seed)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(seed)
+        with pytest.raises(RuntimeError, match="every replay"):
+            drop(x)
+        with pytest.raises(RuntimeError, match="every replay"):
+            join(x, r)
+    seen = []
+    for value in (3, 4):
+        seed.fill_(value)
+        graph.replay()
+        for a, c in zip(out, step(value)):
+            assert torch.equal(a, c)
+        seen.append(out[1].clone())
+    assert not torch.equal(*seen)

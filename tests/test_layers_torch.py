@@ -370,3 +370,16 @@ def test_an_unused_norm_has_no_part_in_gradients(layers):
     gx, gr, gw, gb = torch.autograd.grad(h, leaves, gh, create_graph=True)
     assert torch.equal(gx, layer_oracle.dropout(gh, 0.3, 7, 2)) and torch.equal(gr, gh)
     assert not gw.any() and not gb.any()
+
+
+def test_layers_do_not_draw_seeds_for_a_graph(monkeypatch):
+    """A capture would freeze the drawn seed; the layers say so before anything runs."""
+    class OnGpu:
+        is_cuda, dtype, device, shape = True, torch.float32, torch.device("cuda"), (2, 3)
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="every replay"):
+        serron.Dropout(0.3)(OnGpu())
+    with pytest.raises(RuntimeError, match="every replay"):
+        serron.DropoutAddLayerNorm2d(3, 0.3)(OnGpu(), OnGpu())
+    assert isinstance(serron.Dropout(0.3).eval()(OnGpu()), OnGpu)
