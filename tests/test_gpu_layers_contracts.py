@@ -114,7 +114,7 @@ def test_an_unused_norm_has_no_part_in_gradients(serron, shape, dtype):
 def _scaled_signs(shape, dim, dtype, scale):
     """Signs of equal number in every row (a zero beside them where the length is odd), times a power of two."""
     length = shape[dim]
-    row = torch.cat((torch.ones(length // 2), -torch.ones(length // 2), torch.zeros(length % 2)))
+    row = torch.cat((torch.ones(length // 2), -torch.ones(length // 2), torch.zeros(length % 2))).double()
     moved = [s for d, s in enumerate(shape) if d != dim]
     return (row * scale).expand(*moved, length).movedim(-1, dim).contiguous().to("cuda", dtype)
 
@@ -212,3 +212,126 @@ def test_layers_take_their_seed_from_memory_in_a_graph(serron):
             assert torch.equal(a, c)
         seen.append(out[1].clone())
     assert not torch.equal(*seen)
+
+
+@pytest.mark.parametrize("p", [0.0, 2.0**-32, 1 - 2.0**-32, 1.0])
+@pytest.mark.parametrize("shape", [(2, 10, 5, 5), (1, 67, 3, 7), (3, 1001)])
+def test_join_of_odd_sizes_at_the_ends_of_p(serron, shape, p):
+    """One element an access on maps of 25 and 21 pixels, shifted vectors on rows of 1001."""
+    for dtype in (torch.float32, torch.float16):
+        x, r, gy, gh = (_rand(shape, dtype, k) for k in range(4))
+        w, b = (_rand((shape[1],), torch.float32, k) for k in (5, 6))
+        leaves = [t.requires_grad_() for t in (x, r, w, b)]
+        y, h = serron.dropout_add_layer_norm(*leaves, p=p, seed=8, sequence=3)
+        grads = torch.autograd.grad((y, h), leaves, (gy, gh))
+        with torch.no_grad():
+            assert torch.equal(h, oracle.dropout(x, p, 8, 3, residual=r))
+            ref = oracle.Norm(h, w, b, 1, 1e-5)
+            oracle.within(y, ref.y, ref.y_bound(), "y")
+            (dh, bound), *others = ref.backward(gy, gh)
+            oracle.within(grads[1], dh, bound, "dresidual")
+            for got, (want, off) in zip(grads[2:], others):
+                oracle.within(got, want, off, "dw, db")
+            if p in (0.0, 2.0**-32):  # with 2^-32 the only word below the threshold is 0: none of these
+                assert torch.equal(grads[0], grads[1])
+            if p == 1.0:
+                assert not grads[0].any()
+
+
+def test_operators_are_as_torch_wants_them(serron):
+    """Schemas, fake kernels and autograd registrations against the real kernels."""
+    ops = torch.ops.serron
+    for shape, dim in (((2, 6, 4, 5), 1), ((7, 24), -1)):
+        x = _rand(shape, torch.float32, 1).requires_grad_()
+        if len(shape) == 4:
+            x = x.detach().to(memory_format=torch.channels_last).requires_grad_()
+        w, b = (_rand((shape[dim],), torch.float32, k).requires_grad_() for k in (2, 3))
+        utils = ("test_schema", "test_autograd_registration", "test_faketensor")
+        seed = torch.tensor(5, device="cuda")
+        torch.library.opcheck(ops.layer_norm, (x, w, b, dim, 1e-5), test_utils=utils)
+        torch.library.opcheck(ops.layer_norm, (x, None, None, dim, 1e-5), test_utils=utils)
+        torch.library.opcheck(ops.dropout, (x, x, 1, 0.3, 7, seed, 2), test_utils=utils)
+        torch.library.opcheck(ops.dropout_add_layer_norm, (x, x, w, b, 0.3, 7, None, 2, dim, 1e-5), test_utils=utils)
+
+
+def test_traced_calls_compute(serron):
+    """What a tracer recorded gives another input its own outputs."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def f(x, r, w, b):
+        y, h = serron.dropout_add_layer_norm(serron.layer_norm(x, w, b), r, w, b, p=0.3, seed=5)
+        return serron.dropout(y, 0.2, seed=6, residual=h)
+
+    args, others = ([*(_rand((2, 6, 9, 9), torch.float32, s + k) for k in (1, 2)),
+                     *(_rand((6,), torch.float32, s + k) for k in (3, 4))] for s in (0, 10))
+    for traced in (make_fx(f)(*args), torch.jit.trace(f, tuple(args))):
+        assert torch.equal(traced(*others), f(*others))
+
+
+def test_function_transforms_and_tangents(serron):
+    x, w, b = _rand((5, 8), torch.float32, 1), _rand((8,), torch.float32, 2), _rand((8,), torch.float32, 3)
+
+    def f(v):
+        return serron.dropout(serron.layer_norm(v, w, b, dim=0), 0.3, seed=5).square().sum()
+
+    got = torch.func.vmap(torch.func.grad(f))(x)
+    for row, g in zip(x, got):
+        leaf = row.clone().requires_grad_()
+        assert torch.equal(torch.autograd.grad(f(leaf), leaf)[0], g)
+    with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+        torch.func.jvp(f, (x[0],), (x[1],))
+
+
+def test_backward_follows_its_stream_and_runs_in_threads(serron):
+    """A node runs on the stream of its forward pass, and nodes of other graphs at the same time."""
+    import threading
+
+    x, r, gy, gh = (_rand((8, 32, 40, 40), torch.float32, k) for k in range(4))
+    w, b = (_rand((32,), torch.float32, k) for k in (5, 6))
+    leaves = [t.requires_grad_() for t in (x, r, w, b)]
+
+    def step():
+        outputs = serron.dropout_add_layer_norm(*leaves, p=0.3, seed=5)
+        return torch.autograd.grad(outputs, leaves, (gy, gh))
+
+    want = step()
+    torch.cuda.synchronize()
+    results = {}
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                results[k] = step()
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(4):
+        for a, c in zip(results[k], want):
+            assert torch.equal(a, c)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        late = [t.detach().clone().requires_grad_() for t in leaves]
+        outputs = serron.dropout_add_layer_norm(*late, p=0.3, seed=5)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, c in zip(torch.autograd.grad(outputs, late, (gy, gh)), want):  # from the default stream
+        assert torch.equal(a, c)
+
+
+def test_recomputed_layers_draw_the_same_mask(serron):
+    from torch.utils.checkpoint import checkpoint
+
+    x, r = (_rand((2, 6, 9, 9), torch.float32, k).requires_grad_() for k in (1, 2))
+    join = serron.DropoutAddLayerNorm2d(6, 0.5, device="cuda")
+    grads = []
+    for again in (False, True):
+        torch.manual_seed(3)
+        y, h = checkpoint(join, x, r, use_reentrant=False) if again else join(x, r)
+        grads.append(torch.autograd.grad((y * 2 + h).square().sum(), (x, r, join.weight)))
+    for a, c in zip(*grads):
+        assert torch.equal(a, c)
