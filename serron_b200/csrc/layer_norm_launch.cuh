@@ -7,17 +7,12 @@
 namespace serron {
 
 template <typename T>
-cudaError_t launch_norm(void (*kernel)(NormArgs<T>), const NormPlan& p, size_t shared, const NormArgs<T>& args,
+cudaError_t launch_norm(void (*kernel)(NormArgs<T>), const NormPlan& p, bool backward, const NormArgs<T>& args,
                         cudaStream_t stream) {
-    if (shared > 48 * 1024) {
-        const cudaError_t err =
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
-        if (err != cudaSuccess) return err;
-    }
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(static_cast<unsigned>(p.blocks), p.clusters);
     config.blockDim = dim3(p.tx, p.ty);
-    config.dynamicSmemBytes = shared;
+    config.dynamicSmemBytes = sizeof(float) * plan_shared_floats(p, backward);
     config.stream = stream;
     cudaLaunchAttribute attribute = {};
     attribute.id = cudaLaunchAttributeClusterDimension;
@@ -41,34 +36,29 @@ cudaError_t launch_rows(const NormPlan& p, bool backward, int join, const NormAr
         auto kernel = of_join<T>(join, norm_rows_kernel<T, V, NV, R, kNoJoin, SHIFTED>,
                                  norm_rows_kernel<T, V, NV, R, kHostSeed, SHIFTED>,
                                  norm_rows_kernel<T, V, NV, R, kAnySeed, SHIFTED>);
-        return launch_norm<T>(kernel, p, 0, args, stream);
+        return launch_norm<T>(kernel, p, false, args, stream);
     }
     if constexpr (NV * V <= 16) {
         auto kernel = of_join<T>(join, norm_rows_bwd_kernel<T, V, NV, R, kNoJoin, SHIFTED>,
                                  norm_rows_bwd_kernel<T, V, NV, R, kHostSeed, SHIFTED>,
                                  norm_rows_bwd_kernel<T, V, NV, R, kAnySeed, SHIFTED>);
-        const size_t floats = p.ty > 1 ? size_t(NV) * V * p.tx * p.ty : 0;
-        return launch_norm<T>(kernel, p, sizeof(float) * floats, args, stream);
+        return launch_norm<T>(kernel, p, true, args, stream);
     }
     return cudaErrorInvalidConfiguration;
 }
 
 template <typename T, int V, int NV, bool FULL>
 cudaError_t launch_columns(const NormPlan& p, bool backward, int join, const NormArgs<T>& args, cudaStream_t stream) {
-    // column_totals' scratch for one number a row, for two in a backward pass
-    const size_t floats = (p.ty > 1 || p.clusters > 1) ? (2 * size_t(p.ty) + 2) * p.tx * V : 0;
     if (!backward) {
         auto kernel = of_join<T>(join, norm_columns_kernel<T, V, NV, kNoJoin, FULL>,
                                  norm_columns_kernel<T, V, NV, kHostSeed, FULL>,
                                  norm_columns_kernel<T, V, NV, kAnySeed, FULL>);
-        return launch_norm<T>(kernel, p, sizeof(float) * floats, args, stream);
+        return launch_norm<T>(kernel, p, false, args, stream);
     }
     if constexpr (NV * V * sizeof(T) <= 64) {
         auto kernel = join == kNoJoin ? norm_columns_bwd_kernel<T, V, NV, kNoJoin, FULL>
                                       : norm_columns_bwd_kernel<T, V, NV, kAnySeed, FULL>;
-        // at the end two sums per channel and warp
-        const size_t most = std::max(2 * floats, size_t(NV) * p.ty * (p.tx / 32) * 2);
-        return launch_norm<T>(kernel, p, sizeof(float) * most, args, stream);
+        return launch_norm<T>(kernel, p, true, args, stream);
     }
     return cudaErrorInvalidConfiguration;
 }

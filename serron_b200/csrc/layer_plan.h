@@ -122,4 +122,13 @@ inline NormPlan norm_plan(int64_t rows, int64_t len, int64_t inner, int V, int s
     return p;
 }
 
+// Floats of dynamic shared memory that the plan's kernel takes.  Rows: a backward pass joins the parameters' sums of a
+// block's groups there.  Columns: column_totals' scratch for one number a row, for two in a backward pass, and at its
+// end two sums per channel and warp.  No plan takes more than 48 KB, which need not be asked for.
+inline int64_t plan_shared_floats(const NormPlan& p, bool backward) {
+    if (p.rows) return backward && p.ty > 1 ? int64_t(p.NV) * p.V * p.tx * p.ty : 0;
+    const int64_t totals = (p.ty > 1 || p.clusters > 1) ? (2 * int64_t(p.ty) + 2) * p.tx * p.V : 0;
+    return backward ? std::max(2 * totals, int64_t(p.NV) * p.ty * (p.tx / 32) * 2) : totals;
+}
+
 }  // namespace serron
