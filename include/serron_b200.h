@@ -222,7 +222,9 @@ SERRON_API int serron_derived_forward(int32_t mode, const void* input, const int
  *   - `mean` and `rstd` (outer * inner elements, row (o, i) at o * inner + i; float32, or float64 for
  *     float64 inputs) are what the backward reads; both are NULL where none follows (one alone is refused).
  *   - the backward gives grad_input, grad_weight and grad_bias (the last two of `param_dtype`), each
- *     skipped where NULL, in sums whose order depends on the sizes alone.
+ *     skipped where NULL, in sums of a fixed order: a call repeated gives the same bits.  The sizes set the
+ *     order, and the alignment of the call's pointers, which chooses vectors or single elements: equal
+ *     tensors at other addresses may differ in the last bits.
  *   - workspace: serron_layer_norm_workspace_bytes bytes, 256-byte aligned; -1 (with a message) for
  *     arguments no call takes.
  *   - every tensor starts on a boundary of its elements (a seed in device memory of 8 bytes); other

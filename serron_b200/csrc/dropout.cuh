@@ -13,8 +13,8 @@ namespace serron {
 // half of the first two rounds.  The round keys are operands in constant memory where the seed is the host's.
 //
 // 16-bit elements are bound by the generator: five 32 x 32 -> 64 bit products an element, 17 instructions in all (26 with keys
-// made in the kernel and elements unpacked one at a time).  (64,32,256,256) bfloat16: 104 us (5.2 TB/s, 79 % of the copy
-// rate), with a residual 117 (at the copy rate, part of it from the L2); float32 runs at 90 to 100 % of it.
+// made in the kernel and elements unpacked one at a time).  (64,32,256,256) bfloat16: 103 to 113 us from run to run (72 to
+// 80 % of the copy rate), with a residual 117 (at the copy rate, part of it from the L2); float32 runs at 88 to 100 % of it.
 template <typename T, int V, int U, bool RESIDUAL, bool DEVICE_SEED>
 __global__ void __launch_bounds__(256)
     dropout_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __restrict__ y, long long n,
@@ -73,7 +73,8 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// Any alignment, any type and any `span` (the elements that share a decision), an element at a time.
+// Any alignment, any type and any `span` (the elements that share a decision), an element and a block of the generator at a
+// time: 706 us at (64,32,256,256) bfloat16 an element off the boundary of a vector, seven times the vectors' time.
 template <typename T>
 __global__ void __launch_bounds__(256)
     dropout_any_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __restrict__ y, long long n,

@@ -27,6 +27,11 @@ struct NormShape {
 // kernels for any length and layout: rows are cut into chunks of `chunk` elements, each block reduces one chunk of
 // one row (inner == 1: 256 threads along the row) or of 32 neighbouring rows (inner > 1: 32 x 8 threads, neighbouring
 // rows being neighbours in memory), and the chunks' results are joined where they are used.
+//
+// Bound by loads of single elements, and by reading x three times (twice from DRAM where a chunk stays in the caches) and in
+// a backward pass gy and x three times.  Forward and backward, of the copy rate: (16,32,256,256) float64 205 and 448 us (40
+// and 27 %), (8192,1024) float64 47 and 124 us (44 and 25 %), (400,70000) bfloat16 70 and 168 us (24 and 15 %),
+// (16,2100,32,32) bfloat16 106 and 251 us (20 and 13 %).
 // ------------------------------------------------------------------------------------------------
 constexpr int kNormThreads = 256;
 
@@ -199,7 +204,7 @@ __global__ void __launch_bounds__(kNormThreads)
 
 // ------------------------------------------------------------------------------------------------
 // gradients of weight and bias: sums over rows, first of `rows_per` rows each in A, then of those in double, each in
-// an order that the sizes alone set
+// an order that the sizes set
 // ------------------------------------------------------------------------------------------------
 
 // inner == 1: a thread owns an element of the row and walks down rows_per rows.

@@ -13,12 +13,18 @@
 // level far above the spread costs nothing; the backward pass adds up two numbers once.  Statistics, sums and
 // products are float32; what is stored in 16 bits is rounded once.
 //
-// What bounds them: instructions.  The memory's rate leaves 16-bit elements about 20 instructions each at full issue.  One
-// float at a time the forward pass took 31 an element of a row and 48 of a column; computed on in pairs (layer_vec.cuh),
-// with divisions as one multiplication and one correction, it takes 23 and 15, the backward pass 25 and 24, and the
-// generator adds 19 to 28 in the join.  Warps issue in 52 to 68 % of the cycles (16 to 28 of them are resident).
-//   (64,32,256,256) bfloat16, columns: norm 99 us forward (5.4 TB/s, 83 % of the copy rate of 6.55), 165 backward (74 %);
-//   join 254 (65 %) and 361 (57 %).  (8192,1024) bfloat16, rows: 10.9 and 21.3 us; join 19.9 and 31.6.
+// What bounds them: the latency of loads and of dependent instructions, with too few warps to hide it.  Registers leave
+// room for 14 to 28 warps an SM, which issue in 52 to 68 % of the cycles and wait first for memory (rows, the columns'
+// backward pass) or for the previous instruction (columns forward, the join).  Fewer instructions are therefore time won: the memory's rate leaves 16-bit
+// elements about 20 each at full issue.  One float at a time the forward pass took 31 an element of a row and 48 of a
+// column; computed on in pairs (layer_vec.cuh), with divisions as one multiplication and one correction, it takes 23
+// and 15, the backward pass 25 and 24, and the generator adds 22 to 26 in the join.
+//   (64,32,256,256) bfloat16, columns: norm 98 us forward (5.5 TB/s, 84 % of the copy rate of 6.55), 165 backward (75 %);
+//   join 254 (65 %) and 361 (57 %).  (8192,1024) bfloat16, rows: 10.9 and 21.3 us; join 19.9 and 31.5.
+// The join moves four passes where dropout with a residual and the norm after it move five, but its 41 instructions an
+// element are more than their 18 and 15: of the columns above it takes 254 us, they take 116 + 98; of (32,64,128,128)
+// bfloat16 70 us against 32 + 28.  Of rows it takes what they take: 19.9 us against 10.8 + 10.9, (2048,4096) float16 22.1
+// against 10.4 + 13.5.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -662,7 +668,8 @@ __device__ __forceinline__ Pack<T, V> trimmed(const Pack<T, V>& v, const T* p, b
 }
 
 // Registers: 64 for whole vectors (11.1 us at (8192,1024) bfloat16; at 80, 96, 128 12.2, 12.1, 12.4), 80 in the join, which at 64
-// is slower for short rows (200,000 of 64: 33 us against 30); 32 more where vectors are shifted, which spilled.
+// is slower for short rows (200,000 of 64: 33 us against 30); 32 more where vectors are shifted, of which the kernels of
+// four 16-bit vectors a thread still spill (76 to 92 bytes).  Swept in bfloat16; float32 and single elements take the same.
 template <typename T, int V, int NV, int R, int JOIN, bool SHIFTED>
 __global__ void __maxnreg__((JOIN ? 80 : 64) + (SHIFTED ? 32 : 0))
     norm_rows_kernel(const __grid_constant__ NormArgs<T> a) {

@@ -111,7 +111,11 @@ inline NormPlan norm_plan(int64_t rows, int64_t len, int64_t inner, int V, int s
     const int on_an_sm = p.rows && !backward ? 1024 : 512;
     const int64_t resident = std::max<int64_t>(1, int64_t(kSMs) * std::max(1, on_an_sm / threads) / p.clusters);
     int64_t each = p.tiles <= 2 * resident ? 1 : plan_ceil(p.tiles, resident);
-    if (backward)  // no more than 128 rows to a sum of the parameters' gradients, which keeps those as exact as a tree's
+    // No more than 128 rows (rows) or 256 pairs of a lane's rows (columns: two a tile) to a thread's part of a float32 sum of
+    // the parameters' gradients.  A block adds up its threads' parts in float32 too: the groups one after the other, at
+    // most 128 (rows of up to eight elements); the lanes of a warp as a tree, then its four warps.  So no term takes
+    // part in more than about 270 additions before the sums of the blocks, which are joined in double.
+    if (backward)
         each = std::min<int64_t>(each, 128 / p.R);
     else if (p.rows)  // little is done once a block: rather four rounds of blocks (10.9 us against 14.1)
         each = std::max<int64_t>(1, each / 4);
