@@ -383,3 +383,15 @@ def test_layers_do_not_draw_seeds_for_a_graph(monkeypatch):
     with pytest.raises(RuntimeError, match="every replay"):
         serron.DropoutAddLayerNorm2d(3, 0.3)(OnGpu(), OnGpu())
     assert isinstance(serron.Dropout(0.3).eval()(OnGpu()), OnGpu)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_inference_mode(layers, name):
+    """Below autograd altogether, with tensors from inside and from outside."""
+    f, _ = _functions(layers)[name]
+    outside = _tensors((3, 5, 4), 1)
+    want = f(*outside)
+    with torch.inference_mode():
+        _close(f(*outside), want)
+        _close(f(*(t.clone() for t in outside)), want)
+        assert not f(*outside).requires_grad
