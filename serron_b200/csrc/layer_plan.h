@@ -75,8 +75,9 @@ inline void plan_rows(NormPlan& p, int64_t rows, int64_t len, int size, bool bac
 inline void plan_columns(NormPlan& p, int64_t rows, int64_t len, int64_t inner, int size, bool backward) {
     if (len * inner >= int64_t(1) << 31) return;
     const int64_t columns = rows / p.V;
-    // what fits in registers but for a few spilled words (48 bytes at most): 64 bytes of each tensor, of the one of a forward pass 128 ((64,32,256,256)
-    // bfloat16 forward: 105 us with 16 strides a thread, 147 with 8; backward 165 with 8, 249 with 4)
+    // what fits in registers but for a few spilled words (48 bytes at most): 64 bytes of each tensor, of the one of a
+    // forward pass 128 ((64,32,256,256) bfloat16 forward: 105 us with 16 strides a thread, 147 with 8; backward 165
+    // with 8, 249 with 4)
     int per = p.V == 4 ? std::max(4, (backward ? 8 : 16) / (size / 2)) : 16;
     const int least = p.V == 4 ? 4 : 8;
     while (per > least && (len <= per / 2 || columns * plan_ceil(len, per) < int64_t(kSMs) * 512) &&
